@@ -26,7 +26,7 @@ extern "C" {
 #define LX2V_EUNSUP (-2)   /* valid request outside what the kernels are built for */
 #define LX2V_EHIP (-3)     /* a HIP runtime call failed (launch error) */
 
-/* ABI version of this header (bumped when a signature changes or an entry point is added). */
+/* ABI version of this header (bumped when a signature or the meaning of an argument changes; entry points are only ever added). */
 int lx2v_abi_version(void);
 /* Thread-local text of the last non-zero return. Host pointer, valid until the next call. */
 const char* lx2v_last_error(void);
@@ -409,6 +409,65 @@ int lx2v_gemm_int8_ws(const int8_t* A, int64_t lda, const float* a_scale, const 
                       const float* w_scale, const float* bias, uint16_t* C, int64_t ldc, int64_t M,
                       int64_t N, int64_t K, int epilogue, const uint16_t* resid, int64_t ldr,
                       const float* gate, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ==== Block-scaled e4m3 Linear: one scale per 128 columns of K ================================
+ * The operand form of the reference's "fp8-b128-deepgemm" mm-type (weight in 128 x 128 blocks, activation in groups of
+ * 128 channels per token; lightx2v/common/ops/mm/mm_weight.py): parity unpinned, its kernels live in an absent wheel. */
+
+/* ---- activation operand: scale[r, g] = max(max|x[r, 128 g .. 128 g + 127]|, 1e-12) / 448 ; out = e4m3(x * (1 / scale)) ----
+ * (round to nearest even; both quotients correctly rounded; a row of 128 columns gets the bytes and the scale of
+ * lx2v_quant_fp8_rowwise).  The last group may be short.  Scales are stored group after group: element (r, g) at
+ * scale[g * ld_scale + r], ld_scale >= rows.  NaN elements do not count in the maximum and become NaN codes; an infinite
+ * element makes its group's scale infinite and its own code NaN.  dim % 8 == 0.  `kseg` as in lx2v_quant_fp8_rowwise_kseg,
+ * or NULL.  No counterpart in the reference's sources (its kernel lives in a wheel). */
+int lx2v_quant_fp8_group128(const uint16_t* x, int64_t ldx, const lx2v_kseg* kseg, uint8_t* out, int64_t ldo, float* scale,
+                            int64_t ld_scale, int64_t rows, int dim, void* stream);
+int lx2v_quant_fp8_group128_f32(const float* x, int64_t ldx, uint8_t* out, int64_t ldo, float* scale, int64_t ld_scale,
+                                int64_t rows, int dim, void* stream);
+
+/* ---- weight operand: the same rule over blocks of 128 rows x 128 columns; block (i, g) at scale[i * ld_scale + g],
+ * ld_scale >= ceil(dim / 128): the layout of a checkpoint's block scales.  Edge blocks may be short.  dim % 8 == 0. */
+int lx2v_quant_fp8_block128(const uint16_t* w, int64_t ldw, uint8_t* out, int64_t ldo, float* scale, int64_t ld_scale,
+                            int64_t rows, int dim, void* stream);
+int lx2v_quant_fp8_block128_f32(const float* w, int64_t ldw, uint8_t* out, int64_t ldo, float* scale, int64_t ld_scale,
+                                int64_t rows, int dim, void* stream);
+
+/* ---- C[m, n] = epilogue(sum_b sa[m, b] sw[n / 128, b] (A8[m, b] . W8[n, b]) + bias[n]), bf16 out ----
+ * b runs over the ceil(K / 128) blocks of K; sa[m, b] = a_scale[b * ld_a_scale + m], sw[i, b] = w_scale[i * ld_w_scale + b].
+ * fp32 accumulation; epilogues as lx2v_gemm_bf16, with one rounding at the end (resid may alias C).
+ * K % 16 == 0, N % 8 == 0, e4m3 row strides % 16 and below 4 MiB, any M >= 0.
+ * A product of few output tiles is split along K: fp32 sums of each range in `workspace`
+ * (lx2v_gemm_fp8_block128_workspace_bytes; 0: not split), joined in a fixed order by a second launch, so results repeat
+ * bit for bit.  A NULL, misaligned (16 bytes) or smaller workspace only switches the split off.  Calls that share a workspace must
+ * be ordered (one stream). */
+int64_t lx2v_gemm_fp8_block128_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int lx2v_gemm_fp8_block128(const uint8_t* A, int64_t lda, const float* a_scale, int64_t ld_a_scale, const uint8_t* W, int64_t ldw,
+                           const float* w_scale, int64_t ld_w_scale, const float* bias, uint16_t* C, int64_t ldc, int64_t M,
+                           int64_t N, int64_t K, int epilogue, const uint16_t* resid, int64_t ldr, const float* gate,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- x += y in place, then out = x * rsqrt(mean(x^2) + eps) * w ------------------------------------
+ * The residual addition of a pre-norm layer and the RMSNorm behind it in one pass (over the whole row, as
+ * lx2v_rmsnorm_rope_bf16 with do_norm = 1).  x: the residual stream, bf16 or fp32 rows; y bf16 rows, or NULL (nothing is
+ * added and x is only read); w fp32 [dim] or NULL.  The norm sees the fp32 sum, before it is rounded to x's type.
+ * `out` may alias y, not x.  dim % 8 == 0, dim <= 8192.
+ * The _quant forms leave the normalised row in 8 bits, rounded once from fp32: `form`
+ *   LX2V_QUANT_FP8_ROW      e4m3, scale[r], the rule of lx2v_quant_fp8_rowwise      (operand of lx2v_gemm_fp8)
+ *   LX2V_QUANT_FP8_GROUP128 e4m3, scale[g * ld_scale + r] per 128 columns           (operand of lx2v_gemm_fp8_block128)
+ *   LX2V_QUANT_INT8_ROW     int8, scale[r], the rule of lx2v_quant_int8_rowwise (weight_mode 0)  (operand of lx2v_gemm_int8)
+ * (ld_scale is read for GROUP128 only).  Replaces, where a norm feeds a quantised Linear, RMSWeightSgl.apply and the
+ * activation quantisation behind it  lightx2v/common/ops/norm/rms_norm_weight.py:131-146, mm/mm_weight.py:492-505. */
+#define LX2V_QUANT_FP8_ROW 0
+#define LX2V_QUANT_FP8_GROUP128 1
+#define LX2V_QUANT_INT8_ROW 2
+int lx2v_add_rmsnorm_bf16(uint16_t* x, int64_t ldx, const uint16_t* y, int64_t ldy, const float* w, uint16_t* out, int64_t ldo,
+                          int64_t rows, int dim, float eps, void* stream);
+int lx2v_add_rmsnorm_f32(float* x, int64_t ldx, const uint16_t* y, int64_t ldy, const float* w, uint16_t* out, int64_t ldo,
+                         int64_t rows, int dim, float eps, void* stream);
+int lx2v_add_rmsnorm_quant_bf16(uint16_t* x, int64_t ldx, const uint16_t* y, int64_t ldy, const float* w, void* out, int64_t ldo,
+                                float* scale, int64_t ld_scale, int form, int64_t rows, int dim, float eps, void* stream);
+int lx2v_add_rmsnorm_quant_f32(float* x, int64_t ldx, const uint16_t* y, int64_t ldy, const float* w, void* out, int64_t ldo,
+                               float* scale, int64_t ld_scale, int form, int64_t rows, int dim, float eps, void* stream);
 
 #ifdef __cplusplus
 }

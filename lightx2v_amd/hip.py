@@ -68,6 +68,16 @@ _SIGNATURES = {
     "lx2v_gemm_fp8_ws": [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _P, _P, _I64, _P],
     "lx2v_gemm_int8_ws": [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _P, _P, _I64, _P],
     "lx2v_gemm_w8a8_workspace_bytes": [_I64, _I64, _I64],
+    "lx2v_quant_fp8_group128": [_P, _I64, _P, _P, _I64, _P, _I64, _I64, _I, _P],
+    "lx2v_quant_fp8_group128_f32": [_P, _I64, _P, _I64, _P, _I64, _I64, _I, _P],
+    "lx2v_quant_fp8_block128": [_P, _I64, _P, _I64, _P, _I64, _I64, _I, _P],
+    "lx2v_quant_fp8_block128_f32": [_P, _I64, _P, _I64, _P, _I64, _I64, _I, _P],
+    "lx2v_gemm_fp8_block128": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _P, _P, _I64, _P],
+    "lx2v_gemm_fp8_block128_workspace_bytes": [_I64, _I64, _I64],
+    "lx2v_add_rmsnorm_bf16": [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I, _F, _P],
+    "lx2v_add_rmsnorm_f32": [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I, _F, _P],
+    "lx2v_add_rmsnorm_quant_bf16": [_P, _I64, _P, _I64, _P, _P, _I64, _P, _I64, _I, _I64, _I, _F, _P],
+    "lx2v_add_rmsnorm_quant_f32": [_P, _I64, _P, _I64, _P, _P, _I64, _P, _I64, _I, _I64, _I, _F, _P],
 }
 EXPORTS = tuple(_SIGNATURES) + ("lx2v_abi_version", "lx2v_last_error")
 
@@ -91,7 +101,8 @@ def load() -> ctypes.CDLL:
     for name, argtypes in _SIGNATURES.items():
         fn = getattr(lib, name)
         fn.argtypes = argtypes
-        fn.restype = ctypes.c_int64 if name in ("lx2v_attn_fp8_workspace_bytes", "lx2v_attn_fp8_static_bytes", "lx2v_attn_bf16_workspace_bytes", "lx2v_gemm_bf16_workspace_bytes", "lx2v_gemm_w8a8_workspace_bytes") else ctypes.c_int
+        fn.restype = ctypes.c_int64 if name in ("lx2v_attn_fp8_workspace_bytes", "lx2v_attn_fp8_static_bytes", "lx2v_attn_bf16_workspace_bytes", "lx2v_gemm_bf16_workspace_bytes", "lx2v_gemm_w8a8_workspace_bytes",
+                                                    "lx2v_gemm_fp8_block128_workspace_bytes") else ctypes.c_int
     lib.lx2v_abi_version.restype = ctypes.c_int
     lib.lx2v_last_error.restype = ctypes.c_char_p
     _lib = lib
@@ -754,3 +765,160 @@ def gemm_fp8(a8: torch.Tensor, a_scale: torch.Tensor, w8: torch.Tensor, w_scale:
                                 _ptr(workspace), 0 if workspace is None else workspace.numel(), _stream())
     _check(st, entry)
     return out
+
+
+# ------------------------------------------------------------------------------- block-scaled fp8
+BLOCK = 128  # columns of K (and rows of a weight) that share one scale
+
+
+class QuantGroups(QuantRows):
+    """An activation in the operand form of `gemm_fp8_block`: e4m3 rows `q` [rows, dim] and one fp32 scale per row and
+    128 columns, `scale` [rows, ceil(dim / 128)] (stored group after group), as `quant_fp8_group128` returns them."""
+
+
+def _launch(entry: str, like: torch.Tensor, *args):
+    """Call an entry point on the current stream of the operands' device (which need not be the current device)."""
+    with torch.cuda.device(like.device):
+        _check(getattr(load(), entry)(*args, _stream()), entry)
+
+
+def _need_float_rows(name: str, t: torch.Tensor) -> bool:
+    """bf16 or fp32 GPU [rows, dim] with a contiguous innermost dimension; True for fp32."""
+    if t.dim() != 2:
+        raise Lx2vError(f"{name}: expected [rows, dim], got shape {tuple(t.shape)}")
+    if t.dtype == torch.float32:
+        if not t.is_cuda or (t.stride(1) != 1 and t.shape[1] > 1):
+            raise Lx2vError(f"{name}: fp32 input must be a GPU matrix with a contiguous inner dimension")
+        return True
+    _need_bf16_cuda(name, t)
+    return False
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Row stride as the C ABI wants it: of a tensor with at most one row torch may report anything."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), (t.shape[1] + 15) // 16 * 16)
+
+
+def _group_scales(rows: int, dim: int, device) -> torch.Tensor:
+    """Uninitialised fp32 scales [rows, groups] in the layout of QuantGroups."""
+    return torch.empty(((dim + BLOCK - 1) // BLOCK, rows), dtype=torch.float32, device=device).t()
+
+
+def _group_stride(scale: torch.Tensor) -> int:
+    return scale.stride(1) if scale.shape[1] > 1 else max(scale.shape[0], 1)
+
+
+def quant_fp8_group128(x: torch.Tensor, kseg: Optional["KSeg"] = None, dim: Optional[int] = None):
+    """bf16 / fp32 [rows, dim] -> (e4m3 [rows, dim], fp32 scale [rows, ceil(dim / 128)]): one scale per row and 128 columns,
+    x ~= q * scale.  The scales lie group after group in memory (the tensor is a transposed view).  `kseg` + `dim` as in
+    `quant_fp8_rowwise` (bf16 only)."""
+    f32 = _need_float_rows("quant_fp8_group128.x", x)
+    if f32 and kseg is not None:
+        raise Lx2vError("quant_fp8_group128: a segmented source is bf16")
+    rows = x.shape[0]
+    dim = x.shape[1] if kseg is None else int(dim)
+    q = torch.empty((rows, dim), dtype=torch.float8_e4m3fn, device=x.device)
+    scale = _group_scales(rows, dim, x.device)
+    out = (q.data_ptr(), dim, scale.data_ptr(), _group_stride(scale), rows, dim)
+    if f32:
+        _launch("lx2v_quant_fp8_group128_f32", x, x.data_ptr(), _row_stride(x), *out)
+    else:
+        _launch("lx2v_quant_fp8_group128", x, x.data_ptr(), _row_stride(x), None if kseg is None else ctypes.byref(kseg), *out)
+    return q, scale
+
+
+def quant_fp8_block128(w: torch.Tensor):
+    """bf16 / fp32 weight [N, K] -> (e4m3 [N, K], fp32 scale [ceil(N / 128), ceil(K / 128)]): one scale per 128 x 128 block."""
+    f32 = _need_float_rows("quant_fp8_block128.w", w)
+    rows, dim = w.shape
+    q = torch.empty((rows, dim), dtype=torch.float8_e4m3fn, device=w.device)
+    scale = torch.empty(((rows + BLOCK - 1) // BLOCK, (dim + BLOCK - 1) // BLOCK), dtype=torch.float32, device=w.device)
+    _launch("lx2v_quant_fp8_block128_f32" if f32 else "lx2v_quant_fp8_block128", w, w.data_ptr(), _row_stride(w), q.data_ptr(), dim, scale.data_ptr(), scale.shape[1], rows, dim)
+    return q, scale
+
+
+def gemm_fp8_block_workspace_bytes(M: int, N: int, K: int) -> int:
+    """Bytes of partial sums `gemm_fp8_block` uses for a call of this shape (0: it is not split along K)."""
+    return int(load().lx2v_gemm_fp8_block128_workspace_bytes(int(M), int(N), int(K)))
+
+
+def gemm_fp8_block(a8: torch.Tensor, a_scale: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias=None, epilogue: int = EPI_NONE,
+                   resid: Optional[torch.Tensor] = None, gate=None, out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """(a8 [M,K] e4m3) @ (w8 [N,K] e4m3)^T with a scale per row and 128 columns of K of a8 (`a_scale` [M, ceil(K/128)]) and per
+    128 x 128 block of w8 (`w_scale` [ceil(N/128), ceil(K/128)]) -> epilogue(. + bias) bf16 [M,N].
+    K % 16 == 0, N % 8 == 0.  `a_scale` as `quant_fp8_group128` lays it out is read in place; another layout is copied first.
+    `resid` may be `out`.  `workspace`: uint8 GPU tensor for products that are split along K (`gemm_fp8_block_workspace_bytes`;
+    calls that share one must be ordered on one stream); absent, it comes from torch's allocator when one is needed."""
+    dev = a8.device
+    for n, t in (("a8", a8), ("w8", w8)):
+        if not t.is_cuda or t.device != dev or t.dtype != torch.float8_e4m3fn or t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+            raise Lx2vError(f"gemm_fp8_block: {n} must be a float8_e4m3fn matrix on one GPU with a contiguous inner dimension, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    M, K = a8.shape
+    N = w8.shape[0]
+    if w8.shape[1] != K:
+        raise Lx2vError(f"gemm_fp8_block: K mismatch {K} vs {w8.shape[1]}")
+    groups = (K + BLOCK - 1) // BLOCK
+    for n, t, shape in (("a_scale", a_scale, (M, groups)), ("w_scale", w_scale, ((N + BLOCK - 1) // BLOCK, groups))):
+        if t.device != dev or t.dtype != torch.float32 or tuple(t.shape) != shape:
+            raise Lx2vError(f"gemm_fp8_block: {n} must be fp32 {shape} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if (M > 1 and a_scale.stride(0) != 1) or (groups > 1 and a_scale.stride(1) < M):
+        a_scale = a_scale.t().contiguous().t()
+    if not w_scale.is_contiguous():
+        w_scale = w_scale.contiguous()
+    bias = _vec_f32("gemm_fp8_block.bias", bias, N, a8)
+    gate = _vec_f32("gemm_fp8_block.gate", gate, N, a8)
+    if out is None:
+        out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+    else:
+        _need_out("gemm_fp8_block.out", out, (M, N), a8)
+    if resid is not None:
+        _need_out("gemm_fp8_block.resid", resid, (M, N), a8)
+    elif epilogue == EPI_RESIDUAL:
+        raise Lx2vError("gemm_fp8_block: the residual epilogue needs `resid`")
+    with torch.cuda.device(dev):
+        if workspace is None:
+            need = load().lx2v_gemm_fp8_block128_workspace_bytes(M, N, K)
+            if need > 0:
+                workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        elif workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
+            raise Lx2vError("gemm_fp8_block: workspace must be a contiguous uint8 tensor on the operands' device")
+        st = load().lx2v_gemm_fp8_block128(a8.data_ptr(), _row_stride(a8), a_scale.data_ptr(), _group_stride(a_scale), w8.data_ptr(), _row_stride(w8),
+                                           w_scale.data_ptr(), groups, _ptr(bias), out.data_ptr(), _row_stride(out), M, N, K, epilogue,
+                                           _ptr(resid), 0 if resid is None else _row_stride(resid), _ptr(gate),
+                                           _ptr(workspace), 0 if workspace is None else workspace.numel(), _stream())
+    _check(st, "lx2v_gemm_fp8_block128")
+    return out
+
+
+_NORM_FORMS = {"row": 0, "group": 1, "int8": 2}  # LX2V_QUANT_*
+
+
+def add_rmsnorm_(x: torch.Tensor, y: Optional[torch.Tensor], weight=None, eps: float = 1e-6, out: Optional[torch.Tensor] = None, quant: Optional[str] = None):
+    """x += y in place (x: the residual stream, bf16 or fp32 [rows, dim]; y bf16, or None: nothing is added), then
+    RMSNorm(x) * weight over the whole row, taken from the fp32 sum.  Returns it as bf16 (`out`: its optional destination,
+    which may be y), or quantised from fp32: `quant` = "row" (hip.QuantRows: e4m3, one scale per row, for `gemm_fp8`), "group"
+    (hip.QuantGroups: e4m3, one scale per 128 columns, for `gemm_fp8_block`) or "int8" (hip.QuantRows of int8, for `gemm_int8`)."""
+    f32 = _need_float_rows("add_rmsnorm.x", x)
+    rows, dim = x.shape
+    if y is not None:
+        _need_bf16_cuda("add_rmsnorm.y", y)
+        if y.shape != x.shape or y.device != x.device:
+            raise Lx2vError(f"add_rmsnorm: y {tuple(y.shape)} on {y.device} does not match x {tuple(x.shape)} on {x.device}")
+    w = _vec_f32("add_rmsnorm.weight", weight, dim, x)
+    args = (x.data_ptr(), _row_stride(x), _ptr(y), 0 if y is None else _row_stride(y), _ptr(w))
+    if quant is None:
+        if out is None:
+            out = torch.empty((rows, dim), dtype=torch.bfloat16, device=x.device)
+        else:
+            _need_out("add_rmsnorm.out", out, (rows, dim), x)
+        _launch("lx2v_add_rmsnorm_f32" if f32 else "lx2v_add_rmsnorm_bf16", x, *args, out.data_ptr(), _row_stride(out), rows, dim, eps)
+        return out
+    if out is not None:
+        raise Lx2vError("add_rmsnorm: `out` and `quant` exclude each other")
+    if quant not in _NORM_FORMS:
+        raise Lx2vError(f"add_rmsnorm: quant={quant!r}: None, {', '.join(map(repr, _NORM_FORMS))} are built")
+    q = torch.empty((rows, dim), dtype=torch.int8 if quant == "int8" else torch.float8_e4m3fn, device=x.device)
+    scale = _group_scales(rows, dim, x.device) if quant == "group" else torch.empty((rows,), dtype=torch.float32, device=x.device)
+    _launch("lx2v_add_rmsnorm_quant_f32" if f32 else "lx2v_add_rmsnorm_quant_bf16", x, *args, q.data_ptr(), dim, scale.data_ptr(),
+            _group_stride(scale) if quant == "group" else 0, _NORM_FORMS[quant], rows, dim, eps)
+    return (QuantGroups if quant == "group" else QuantRows)(q, scale)

@@ -1,0 +1,84 @@
+"""Refusals of the block-scaled e4m3 Linear, its quantisers and the residual RMSNorm: nothing is launched, no GPU is needed."""
+import ctypes
+
+import pytest
+import torch
+
+from lightx2v_amd import hip
+from oracle import fp8_block_ref as R
+
+
+@pytest.fixture(scope="module")
+def p():
+    buf = ctypes.create_string_buffer(4096 + 16)
+    yield (ctypes.addressof(buf) + 15) & ~15
+    del buf
+
+
+def _gemm(p, **kw):
+    a = dict(A=p, lda=128, sa=p, lsa=64, W=p, ldw=128, sw=p, lsw=1, bias=None, C=p, ldc=64, M=8, N=64, K=128, epi=0, resid=None, ldr=0, gate=None, ws=None, wsb=0, st=None)
+    a.update(kw)
+    return hip.load().lx2v_gemm_fp8_block128(*a.values())
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(A=None), -1, b"null"), (dict(sa=None), -1, b"null"), (dict(sw=None), -1, b"null"), (dict(C=None), -1, b"null"),
+    (dict(M=-1), -1, b"bad shape"), (dict(N=0), -1, b"bad shape"), (dict(K=0), -1, b"bad shape"), (dict(M=1 << 31, lsa=1 << 31), -2, b"31 bits"),
+    (dict(K=120), -2, b"multiple of 16"), (dict(N=60), -2, b"of 8"), (dict(lda=136), -1, b"multiples of 16"), (dict(ldc=66), -1, b"ldc of 8"),
+    (dict(lda=112), -1, b"smaller"), (dict(ldw=112), -1, b"smaller"), (dict(ldc=56), -1, b"smaller"), (dict(lda=1 << 22), -2, b"4 MiB"),
+    (dict(lsa=7), -1, b"ld_a_scale"), (dict(K=256, lda=256, ldw=256), -1, b"ld_w_scale"), (dict(lsw=1 << 28), -2, b"too large"), (dict(epi=3), -1, b"unknown epilogue"), (dict(epi=2), -1, b"resid")])
+def test_gemm_refuses(p, kw, code, text):
+    assert _gemm(p, **kw) == code
+    assert text in hip.load().lx2v_last_error(), hip.load().lx2v_last_error()
+
+
+def test_gemm_refuses_misaligned_tensors(p):
+    for name, off in (("A", 8), ("W", 8), ("C", 8), ("bias", 4), ("sa", 2), ("sw", 1)):
+        assert _gemm(p, **{name: p + off}) == -1 and b"aligned" in hip.load().lx2v_last_error()
+    for kw in (dict(resid=p + 8, ldr=64), dict(resid=p, ldr=60), dict(resid=p, ldr=56), dict(resid=p, ldr=64, gate=p + 4)):
+        assert _gemm(p, epi=2, **kw) == -1
+    assert _gemm(p, M=0) == 0   # nothing to do
+    assert _gemm(p, M=0, A=None, W=None, C=None, sa=None, sw=None) == 0
+
+
+def test_quantisers_and_norm_refuse(p):
+    lib = hip.load()
+    assert lib.lx2v_quant_fp8_group128(None, 128, None, p, 128, p, 4, 4, 128, None) == -1
+    assert lib.lx2v_quant_fp8_group128(p, 128, None, p, 128, p, 4, 4, 124, None) == -1       # dim % 8
+    assert lib.lx2v_quant_fp8_group128(p, 128, None, p, 128, p, 3, 4, 128, None) == -1       # scales overlap
+    assert lib.lx2v_quant_fp8_group128(p, 120, None, p, 128, p, 4, 4, 128, None) == -1       # source rows overlap
+    assert lib.lx2v_quant_fp8_group128(p + 2, 128, None, p, 128, p, 4, 4, 128, None) == -1
+    bad = hip.KSeg(seg=64, stride=64, split=32, seg2=64, stride2=64, base2=0, lda2=64)
+    assert lib.lx2v_quant_fp8_group128(p, 128, ctypes.byref(bad), p, 128, p, 4, 4, 128, None) == -1
+    assert lib.lx2v_quant_fp8_group128(p, 128, None, p, 128, p, 0, 0, 128, None) == 0
+    assert lib.lx2v_quant_fp8_block128(p, 128, p, 128, p, 0, 4, 128, None) == -1              # scale stride
+    assert lib.lx2v_quant_fp8_block128(p, 128, p, 128, p, 1, 0, 128, None) == 0
+    assert lib.lx2v_add_rmsnorm_bf16(p, 64, p, 64, None, p, 64, 4, 64, 1e-6, None) == -1 and b"out may not be x" in lib.lx2v_last_error()
+    assert lib.lx2v_add_rmsnorm_bf16(p, 64, p, 64, None, p + 64, 64, 4, 8200, 1e-6, None) == -2
+    assert lib.lx2v_add_rmsnorm_bf16(p, 64, p, 64, None, p + 64, 64, 4, 60, 1e-6, None) == -2
+    assert lib.lx2v_add_rmsnorm_f32(p, 64, p, 56, None, p + 64, 64, 4, 64, 1e-6, None) == -1
+    assert lib.lx2v_add_rmsnorm_f32(p, 64, p, 64, p + 4, p + 64, 64, 4, 64, 1e-6, None) == -1
+    for form in (-1, 3):
+        assert lib.lx2v_add_rmsnorm_quant_bf16(p, 64, p, 64, None, p + 64, 64, p, 4, form, 4, 64, 1e-6, None) == -1 and b"form" in lib.lx2v_last_error()
+    assert lib.lx2v_add_rmsnorm_quant_bf16(p, 64, p, 64, None, p + 64, 64, None, 4, 0, 4, 64, 1e-6, None) == -1
+    assert lib.lx2v_add_rmsnorm_quant_bf16(p, 64, p, 64, None, p + 64, 64, p, 3, 1, 4, 64, 1e-6, None) == -1   # scales overlap
+    assert lib.lx2v_add_rmsnorm_quant_bf16(p, 64, p, 64, None, p + 64, 64, p, 0, 1, 0, 64, 1e-6, None) == 0
+
+
+def test_python_refuses_cpu_tensors_and_wrong_types():
+    x = torch.zeros(4, 128, dtype=torch.bfloat16)
+    q, s = R.quantise(x, 1)
+    for call in (lambda: hip.quant_fp8_group128(x), lambda: hip.quant_fp8_block128(x), lambda: hip.add_rmsnorm_(x, x), lambda: hip.gemm_fp8_block(q, s, q, s),
+                 lambda: hip.quant_fp8_group128(x.float()), lambda: hip.add_rmsnorm_(x.float(), x), lambda: hip.quant_fp8_block128(x.half())):
+        with pytest.raises(hip.Lx2vError):
+            call()
+
+
+def test_oracle_quantisation_is_within_half_a_step():
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(200, 400, generator=g) * torch.exp(torch.randn(200, 1, generator=g))
+    for rows in (1, 128):
+        q, s = R.quantise(x, rows)
+        d = R.dequantise(q, s, rows)
+        grid = R.dequantise(torch.ones_like(x).to(torch.float8_e4m3fn), s, rows)
+        assert bool(((d - x.double()).abs() <= torch.maximum(2.0 ** -4 * x.double().abs(), 2.0 ** -10 * grid) * (1 + 2.0 ** -20)).all())
