@@ -25,6 +25,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int BK = 128;
+constexpr int GROUP_M = 4;  // row panels that share one sweep over the columns
 constexpr int EPI_PARTIAL = 3;  // kernel instance that leaves the fp32 sums of a K range in the workspace (internal)
 
 struct Params {
@@ -40,6 +41,7 @@ struct Params {
   int64_t lda, ldw, ldc, ldr, lds_a, lds_w;
   int M, N, K;
   int tiles_m, tiles_n;
+  uint32_t group_rcp;  // floor(2^32 / (GROUP_M * tiles_n))
   int nk;          // K blocks
   int split, per;  // K ranges and K blocks in each
 };
@@ -132,7 +134,6 @@ __global__ __launch_bounds__(256) void gemm_fp8_block_tile_kernel(const Params p
 
   const int item = xcd_remap(blockIdx.x, gridDim.x);
   const int part = item % p.split, tile = item / p.split;
-  constexpr int GROUP_M = 4;  // row panels that share one sweep over the columns
   const int group_sz = GROUP_M * p.tiles_n, first_m = tile / group_sz * GROUP_M;
   const int gm = min(p.tiles_m - first_m, GROUP_M), in_g = tile % group_sz;
   const int m0 = (first_m + in_g % gm) * T::TM, n0 = in_g / gm * T::TN;
@@ -154,7 +155,7 @@ __global__ __launch_bounds__(256) void gemm_fp8_block_tile_kernel(const Params p
   set_voff(false);
   const u32x4 a_rs = raw_descriptor(p.A + (int64_t)m0 * p.lda, min((int64_t)p.M - m0, (int64_t)T::TM) * p.lda);
   const u32x4 w_rs = raw_descriptor(p.W + (int64_t)n0 * p.ldw, min((int64_t)p.N - n0, (int64_t)T::TN) * p.ldw);
-  const bool sw_wave = wid == 3, sa_wave = wid < T::TM / 64;
+  const bool sw_wave = wid == 3, sa_wave = wid < (T::TM + 63) / 64;
   const int nb = min(((p.N + 127) >> 7) - (n0 >> 7), (T::TN + 127) / 128);  // weight row blocks of the tile
   const int s_pv = sw_wave ? (lane < nb ? lane * (int)p.lds_w * 4 : NOWHERE) : sa_wave ? (64 * wid + lane) * 4 : NOWHERE;
 
@@ -237,6 +238,329 @@ __global__ __launch_bounds__(256) void gemm_fp8_block_tile_kernel(const Params p
       else finish4<EPI>(p, acc[i][k], m, n);
     }
   }
+}
+
+// ---- stream kernel ------------------------------------------------------------------------------------
+// Long products: one wave per SIMD, 4 waves (2 x 2), wave tile 16 MT x 128 (one row block of weight scales), persistent: a
+// workgroup walks its output tiles as one stream of K blocks.  Three stages: block j + 2 is on its way into LDS, block
+// j + 1 is read from LDS into fragment registers, block j is multiplied -- fragments are double-buffered in registers, so
+// the LDS reads are spread over the whole block and only two LDS slots are needed.
+// LDS: A slot 0, 1 | W slot 0, 1 | scales 0, 1.
+template <int MT>
+struct Stream {
+  static constexpr int TM = 32 * MT, TN = 256;
+  static constexpr int A_BYTES = TM * BK, W_BYTES = TN * BK;
+  static constexpr int W_AT = 2 * A_BYTES, S_AT = W_AT + 2 * W_BYTES;
+  static constexpr int LDS = S_AT + 2 * 1024;
+  static constexpr int PA = TM / 32, PW = TN / 32;
+  static constexpr int STEPS = 8 * MT;
+  static_assert(STEPS % 3 == 0, "the ring of three results wraps with the block");
+  static constexpr int STORES = 4 * MT;
+};
+
+// n / d and n % d from floor(2^32 / d): the estimate is the quotient or one less.
+LX2V_DEVICE void divmod(uint32_t n, uint32_t d, uint32_t rcp, uint32_t& q, uint32_t& r) {
+  q = __umulhi(n, rcp);
+  r = n - q * d;
+  if (r >= d) {
+    ++q;
+    r -= d;
+  }
+}
+
+template <class P>
+LX2V_DEVICE void tile_origin(P p, int vbid, int tm, int tn, int& m0, int& n0) {
+  const uint32_t t = (uint32_t)xcd_remap(vbid, p->tiles_m * p->tiles_n);
+  uint32_t g, in_g, row, col;
+  divmod(t, (uint32_t)(GROUP_M * p->tiles_n), p->group_rcp, g, in_g);
+  const uint32_t gm = (uint32_t)min(p->tiles_m - (int)g * GROUP_M, GROUP_M);
+  divmod(in_g, gm, gm == 4 ? 0x40000000u : gm == 3 ? 0x55555555u : gm == 2 ? 0x80000000u : 0xffffffffu, col, row);
+  m0 = (int)(g * GROUP_M + row) * tm;
+  n0 = (int)col * tn;
+}
+
+// The kernel's arguments, read again from memory: what a kernel needs once per output tile only would otherwise occupy scalar
+// registers throughout its K loop.
+typedef const __attribute__((address_space(4))) Params* ParamsAgain;
+LX2V_DEVICE ParamsAgain params_again() {
+  uint64_t a = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(a));
+  return reinterpret_cast<ParamsAgain>(a);
+}
+
+// Accumulator registers a32 .. a255 hold the stream kernel's fragments by name (tools/check_mfma_hazards.py checks that the
+// compiler keeps its hands off them).
+#define FRAG_CLOBBERS \
+  "a32", "a33", "a34", "a35", "a36", "a37", "a38", "a39", "a40", "a41", "a42", "a43", "a44", "a45", "a46", "a47", \
+  "a48", "a49", "a50", "a51", "a52", "a53", "a54", "a55", "a56", "a57", "a58", "a59", "a60", "a61", "a62", "a63", \
+  "a64", "a65", "a66", "a67", "a68", "a69", "a70", "a71", "a72", "a73", "a74", "a75", "a76", "a77", "a78", "a79", \
+  "a80", "a81", "a82", "a83", "a84", "a85", "a86", "a87", "a88", "a89", "a90", "a91", "a92", "a93", "a94", "a95", \
+  "a96", "a97", "a98", "a99", "a100", "a101", "a102", "a103", "a104", "a105", "a106", "a107", "a108", "a109", "a110", "a111", \
+  "a112", "a113", "a114", "a115", "a116", "a117", "a118", "a119", "a120", "a121", "a122", "a123", "a124", "a125", "a126", "a127", \
+  "a128", "a129", "a130", "a131", "a132", "a133", "a134", "a135", "a136", "a137", "a138", "a139", "a140", "a141", "a142", "a143", \
+  "a144", "a145", "a146", "a147", "a148", "a149", "a150", "a151", "a152", "a153", "a154", "a155", "a156", "a157", "a158", "a159", \
+  "a160", "a161", "a162", "a163", "a164", "a165", "a166", "a167", "a168", "a169", "a170", "a171", "a172", "a173", "a174", "a175", \
+  "a176", "a177", "a178", "a179", "a180", "a181", "a182", "a183", "a184", "a185", "a186", "a187", "a188", "a189", "a190", "a191", \
+  "a192", "a193", "a194", "a195", "a196", "a197", "a198", "a199", "a200", "a201", "a202", "a203", "a204", "a205", "a206", "a207", \
+  "a208", "a209", "a210", "a211", "a212", "a213", "a214", "a215", "a216", "a217", "a218", "a219", "a220", "a221", "a222", "a223", \
+  "a224", "a225", "a226", "a227", "a228", "a229", "a230", "a231", "a232", "a233", "a234", "a235", "a236", "a237", "a238", "a239", \
+  "a240", "a241", "a242", "a243", "a244", "a245", "a246", "a247", "a248", "a249", "a250", "a251", "a252", "a253", "a254", "a255"
+
+template <int MT, int EPI>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void gemm_fp8_block_stream_kernel(const Params p) {
+  using T = Stream<MT>;
+  __shared__ __attribute__((aligned(16))) char lds[T::LDS];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wid >> 1, wn = wid & 1;
+  const int fr = lane & 15, fq = lane >> 4;
+  const int ntiles = p.tiles_m * p.tiles_n, grid = gridDim.x, nk = p.nk;
+  const int my_tiles = (int)blockIdx.x < ntiles ? (ntiles - 1 - (int)blockIdx.x) / grid + 1 : 0;
+  const int64_t total = (int64_t)my_tiles * nk;
+  if (total == 0) return;
+
+  const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t)(size_t)(__attribute__((address_space(3))) char*)lds);
+  constexpr int NOWHERE = (int)0x80000000u;
+  const bool sw_wave = wid == 3, sa_wave = wid < (T::TM + 63) / 64;
+
+  // ---- DMA cursor: two blocks ahead of the multiplied one ----
+  // piece q of wave w: rows 32 q + 8 w + (lane >> 3) of the operand tile; the swizzle is the same for all q
+  const int chunk = (lane & 7) ^ ((4 * wid + (lane >> 4)) & 7);
+  const int left = p.K - (nk - 1) * BK;  // columns of the last block
+  int a_pv, w_pv;
+  auto set_voff = [&](bool last) __attribute__((always_inline)) {
+    const int r = 8 * wid + (lane >> 3);
+    const bool out = last && chunk * 16 >= left;
+    a_pv = out ? NOWHERE : r * (int)p.lda + chunk * 16;
+    w_pv = out ? NOWHERE : r * (int)p.ldw + chunk * 16;
+  };
+  set_voff(nk == 1);
+  int d_ord = 0, d_kt = 0, s_pv = NOWHERE;
+  uint32_t d_soff = 0;
+  u32x4 a_rs, w_rs, s_rs;
+  uint32_t s_step_lo = 0, s_step_hi = 0;  // bytes from the scales of one block to the next
+  auto d_tile = [&]() __attribute__((always_inline)) {  // descriptors of the cursor's output tile; past the last one they are empty
+    const ParamsAgain p = params_again();
+    const int vbid = d_ord * grid + (int)blockIdx.x;
+    const bool live = vbid < ntiles;
+    int m0 = 0, n0 = 0;
+    if (live) tile_origin(p, vbid, T::TM, T::TN, m0, n0);
+    a_rs = raw_descriptor(p->A + (int64_t)m0 * p->lda, live ? min((int64_t)p->M - m0, (int64_t)T::TM) * p->lda : 0);
+    w_rs = raw_descriptor(p->W + (int64_t)n0 * p->ldw, live ? min((int64_t)p->N - n0, (int64_t)T::TN) * p->ldw : 0);
+    const int nb = min(((p->N + 127) >> 7) - (n0 >> 7), 2);
+    const float* sb = sw_wave ? p->w_scale + (int64_t)(n0 >> 7) * p->lds_w : p->a_scale + m0;
+    s_rs = raw_descriptor(sb, !live ? 0 : sw_wave ? ((int64_t)(nb - 1) * p->lds_w + 1) * 4 : sa_wave ? ((int64_t)p->M - m0) * 4 : 0);
+    s_pv = sw_wave ? (lane < nb ? lane * (int)p->lds_w * 4 : NOWHERE) : (64 * wid + lane) * 4;
+  };
+  d_tile();
+  {
+    const int64_t step = sw_wave ? 4 : p.lds_a * 4;
+    s_step_lo = __builtin_amdgcn_readfirstlane((uint32_t)step);
+    s_step_hi = __builtin_amdgcn_readfirstlane((uint32_t)(step >> 32));
+  }
+  uint32_t dma_base = lds_base + 1024 * (uint32_t)wid, dma_sc = lds_base + 256 * (uint32_t)wid;
+  auto dma16 = [&](auto dstc, const u32x4& rs, int voff, uint32_t soff) __attribute__((always_inline)) {  // (the immediate in the M0 write: no register per target)
+    const uint32_t base = dma_base;
+    asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(base), "v"(voff), "s"(rs), "s"(soff), "i"(decltype(dstc)::value) : "memory", "scc");
+  };
+  auto dma4 = [&](auto dstc, const u32x4& rs, int voff) __attribute__((always_inline)) {
+    const uint32_t base = dma_sc;
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(base), "v"(voff), "s"(rs), "i"(decltype(dstc)::value) : "memory", "scc");
+  };
+  const int a_step = 32 * (int)p.lda, w_step = 32 * (int)p.ldw;
+  auto dma = [&](auto Pc, auto qc) __attribute__((always_inline)) {  // piece q of the cursor's block into slot P: the weight's, the activation's, the scales
+    constexpr int P = decltype(Pc)::value, q = decltype(qc)::value;
+    if constexpr (q < T::PW) dma16(IntC<T::W_AT + P * T::W_BYTES + 4096 * q>{}, w_rs, w_pv + q * w_step, d_soff);
+    else if constexpr (q < T::PW + T::PA) dma16(IntC<P * T::A_BYTES + 4096 * (q - T::PW)>{}, a_rs, a_pv + (q - T::PW) * a_step, d_soff);
+    else dma4(IntC<T::S_AT + P * 1024>{}, s_rs, s_pv);
+  };
+  constexpr int PIECES = T::PW + T::PA + 1;
+  auto d_advance = [&]() __attribute__((always_inline)) {
+    const uint32_t lo = s_rs[0] + s_step_lo;
+    s_rs[1] += s_step_hi + (lo < s_step_lo ? 1u : 0u);
+    s_rs[0] = lo;
+    ++d_kt;
+    d_soff += BK;
+    if (d_kt == nk - 1) {
+      if (left < BK) set_voff(true);
+    }
+    if (d_kt == nk) {
+      if (left < BK) set_voff(nk == 1);
+      d_kt = 0;
+      d_soff = 0;
+      ++d_ord;
+      d_tile();
+    }
+    asm volatile("" : "+s"(a_rs), "+s"(w_rs), "+s"(s_rs), "+s"(dma_base), "+s"(dma_sc));
+  };
+
+  // ---- fragments: register set P (0 | 1) = 8 W fragments, then MT A fragments, of 8 accumulator registers each ----
+  int rd_a[2], rd_w[2];  // LDS addresses of the lane's two 16-byte halves at row block 0
+  {
+    const int ar = wm * 16 * MT + fr, wr = wn * 128 + fr;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      rd_a[c] = (int)lds_base + ar * BK + (((2 * fq + c) ^ ((ar >> 1) & 7)) << 4);
+      rd_w[c] = (int)lds_base + T::W_AT + wr * BK + (((2 * fq + c) ^ ((wr >> 1) & 7)) << 4);
+    }
+  }
+  const char* rd_s = lds + T::S_AT + (wm * 16 * MT + fr) * 4;
+  const char* rd_sw = lds + T::S_AT + 768 + wn * 4;
+  constexpr int FRAG0 = 32, SET = 8 * (8 + MT);
+  static_assert(FRAG0 + 2 * SET <= 256, "fragments exceed the accumulator registers");
+  float sa[MT], sw, s[MT], s_last;
+  f32x4 acc[MT][8];
+  f32x4 part[3];
+  // `old`, the result of the MFMA two before: handed through the statement, so that its additions stay behind this one --
+  // 64 cycles at least after the instruction that made it, which the compiler, not knowing what it is, would not wait for
+  auto mm = [&](f32x4& d, f32x4& old, auto wc, auto ac) __attribute__((always_inline)) {
+    asm volatile("v_mfma_f32_16x16x128_f8f6f4 %0, a[%2:%3], a[%4:%5], 0"
+                 : "=&v"(d), "+v"(old) : "n"(decltype(wc)::value), "n"(decltype(wc)::value + 7), "n"(decltype(ac)::value), "n"(decltype(ac)::value + 7));
+  };
+  auto add = [&](auto tc, float sc) __attribute__((always_inline)) {
+    constexpr int t = decltype(tc)::value;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[t / 8][t % 8][e] = __builtin_fmaf(part[t % 3][e], sc, acc[t / 8][t % 8][e]);
+    asm volatile("" : "+v"(acc[t / 8][t % 8]));  // (pinned here: without a use the sums would sink to the end of the block and keep every result alive)
+  };
+  auto lds_frag = [&](int addr, auto dstc, auto ofsc) __attribute__((always_inline)) {  // 16 bytes a lane into four accumulator registers; waited for at the next barrier
+    asm volatile("ds_read_b128 a[%1:%2], %0 offset:%3" ::"v"(addr), "n"(decltype(dstc)::value), "n"(decltype(dstc)::value + 3), "n"(decltype(ofsc)::value) : "memory", FRAG_CLOBBERS);
+  };
+  // LDS read r of a block from slot P into register set P: 16 halves of W, 2 MT of A, MT + 1 scales
+  auto rd = [&](auto Pc, auto rc) __attribute__((always_inline)) {
+    constexpr int P = decltype(Pc)::value, r = decltype(rc)::value;
+    if constexpr (r < 16) lds_frag(rd_w[r & 1], IntC<FRAG0 + P * SET + 4 * r>{}, IntC<P * T::W_BYTES + (r >> 1) * 2048>{});
+    else if constexpr (r < 16 + 2 * MT) lds_frag(rd_a[r & 1], IntC<FRAG0 + P * SET + 4 * r>{}, IntC<P * T::A_BYTES + ((r - 16) >> 1) * 2048>{});
+    else if constexpr (r < 16 + 3 * MT) sa[r - 16 - 2 * MT] = *reinterpret_cast<const float*>(rd_s + P * 1024 + (r - 16 - 2 * MT) * 64);
+    else if constexpr (r == 16 + 3 * MT) sw = *reinterpret_cast<const float*>(rd_sw + P * 1024);
+  };
+  constexpr int READS = 17 + 3 * MT;
+
+  // One block: multiply register set P, read the next one's fragments from slot 1 - P, stage the one after into slot P.
+  auto block = [&](auto Pc, bool relaxed) __attribute__((always_inline)) {
+    constexpr int P = decltype(Pc)::value, Q = 1 - P;
+    // the next block is complete in LDS once every wave is past this barrier, and every wave has read its fragments of this one
+    if (relaxed) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::STORES) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    s_last = s[MT - 1];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) s[i] = sa[i] * sw;
+    static_for<0, T::STEPS>([&](auto tc) __attribute__((always_inline)) {
+      constexpr int t = decltype(tc)::value;
+      mm(part[t % 3], part[(t + 1) % 3], IntC<FRAG0 + P * SET + 8 * (t % 8)>{}, IntC<FRAG0 + P * SET + 64 + 8 * (t / 8)>{});
+      if constexpr (t >= 2) add(IntC<t - 2>{}, s[(t - 2) / 8]);
+      else add(IntC<T::STEPS - 2 + t>{}, s_last);  // the previous block's last two
+      if constexpr (t < PIECES) dma(IntC<P>{}, IntC<t>{});
+      static_for<t * READS / (T::STEPS - 4), (t + 1) * READS / (T::STEPS - 4)>([&](auto rc) __attribute__((always_inline)) {
+        if constexpr (decltype(rc)::value < READS) rd(IntC<Q>{}, rc);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    d_advance();
+  };
+
+  // ---- epilogue: a lane's four columns become eight consecutive ones by swapping lane rows between two column blocks;
+  // 16-byte stores through a descriptor of the tile's rows: rows past M and columns past N are dropped ----
+  auto epilogue = [&](int m0, int n0) __attribute__((always_inline)) {
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" : "+v"(part[0]), "+v"(part[1]), "+v"(part[2]));  // the last MFMAs were issued a few cycles ago
+    add(IntC<T::STEPS - 2>{}, s[MT - 1]);
+    add(IntC<T::STEPS - 1>{}, s[MT - 1]);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) part[i] = f32x4{0.f, 0.f, 0.f, 0.f};  // the next block adds its predecessor's last two once more
+    const ParamsAgain p = params_again();
+    int fr_ = fr, fq_ = fq;
+    asm volatile("" : "+v"(fr_), "+v"(fq_));
+    const u32x4 c_d = raw_descriptor(p->C + (int64_t)m0 * p->ldc, (min((int64_t)p->M - m0, (int64_t)T::TM) - 1) * p->ldc * 2 + (int64_t)p->N * 2);
+    void* cb = reinterpret_cast<void*>(((uint64_t)c_d[1] << 32) | c_d[0]);
+    const __amdgpu_buffer_rsrc_t c_rs = __builtin_amdgcn_make_buffer_rsrc(cb, 0, (int)c_d[2], 0x00020000);
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+      f32x4 bv[2], gv[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int n = min(n0 + wn * 128 + (k + h) * 16 + fq_ * 4, p->N - 4);
+        bv[h] = p->bias != nullptr ? *reinterpret_cast<const f32x4*>(p->bias + n) : f32x4{0.f, 0.f, 0.f, 0.f};
+        gv[h] = EPI == LX2V_EPI_RESIDUAL && p->gate != nullptr ? *reinterpret_cast<const f32x4*>(p->gate + n) : f32x4{1.f, 1.f, 1.f, 1.f};
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int row = wm * 16 * MT + i * 16 + fr_;
+        uint32_t d[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = acc[i][k + h][e] + bv[h][e];
+            if constexpr (EPI == LX2V_EPI_GELU_TANH) v[e] = gelu_tanh(v[e]);
+            if constexpr (EPI == LX2V_EPI_RESIDUAL) v[e] *= gv[h][e];
+          }
+          if constexpr (EPI == LX2V_EPI_RESIDUAL) {
+            const int m = min(m0 + row, p->M - 1), n = min(n0 + wn * 128 + (k + h) * 16 + fq_ * 4, p->N - 4);
+            const u32x2 r = *reinterpret_cast<const u32x2*>(p->resid + (int64_t)m * p->ldr + n);
+            v[0] += __uint_as_float(r[0] << 16);
+            v[1] += __uint_as_float(r[0] & 0xffff0000u);
+            v[2] += __uint_as_float(r[1] << 16);
+            v[3] += __uint_as_float(r[1] & 0xffff0000u);
+          }
+          d[h][0] = pack2(v[0], v[1]);
+          d[h][1] = pack2(v[2], v[3]);
+          acc[i][k + h] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        // lane rows fq = 0 .. 3 of block k: columns 4 fq ..; swapping the odd rows of d[0] with the even rows of d[1] leaves row 0
+        // with columns 0-7 of block k, row 1 with 0-7 of block k + 1, row 2 with 8-15 of block k, row 3 with 8-15 of block k + 1
+        const auto x = __builtin_amdgcn_permlane16_swap(d[0][0], d[1][0], false, false);
+        const auto y = __builtin_amdgcn_permlane16_swap(d[0][1], d[1][1], false, false);
+        const int n = n0 + wn * 128 + (k + (fq_ & 1)) * 16 + (fq_ >> 1) * 8;
+        const bool in = m0 + row < p->M && n < p->N;
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], y[0], x[1], y[1]}, c_rs, in ? (row * (int)p->ldc + n) * 2 : NOWHERE, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // ---- prologue: blocks 0 and 1 staged, fragments of block 0 ----
+  static_for<0, PIECES>([&](auto qc) __attribute__((always_inline)) { dma(IntC<0>{}, qc); });
+  d_advance();
+  static_for<0, PIECES>([&](auto qc) __attribute__((always_inline)) { dma(IntC<1>{}, qc); });
+  d_advance();
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  static_for<0, READS>([&](auto rc) __attribute__((always_inline)) { rd(IntC<0>{}, rc); });
+#pragma unroll
+  for (int i = 0; i < 3; ++i) part[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < MT; ++i) s[i] = 0.f;
+
+  int ord = 0, kt = 0;
+  bool relaxed = false;
+  auto after = [&]() __attribute__((always_inline)) {
+    relaxed = false;
+    if (++kt == nk) {
+      int m0, n0;
+      tile_origin(params_again(), ord * grid + (int)blockIdx.x, T::TM, T::TN, m0, n0);
+      epilogue(m0, n0);
+      relaxed = true;
+      kt = 0;
+      ++ord;
+    }
+  };
+  for (int64_t j = 0; j < total; j += 2) {
+    block(IntC<0>{}, relaxed);
+    after();
+    if (j + 1 < total) {
+      block(IntC<1>{}, relaxed);
+      after();
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA may still be writing this workgroup's LDS when it ends
 }
 
 // Sum of the K ranges in their order, then the epilogue: four columns per thread.
@@ -357,7 +681,9 @@ void launch(const Params& p, Kind kind, hipStream_t st) {
       return;
     case TILE_64x128: return launch_tile<2, 4, 3, EPI>(p, items, st);
     case TILE_128x128: return launch_tile<4, 4, 2, EPI>(p, items, st);
-    default: return launch_tile<6, 8, 2, EPI>(p, items, st);
+    default:
+      if constexpr (EPI != EPI_PARTIAL) hipLaunchKernelGGL((gemm_fp8_block_stream_kernel<6, EPI>), dim3((unsigned)std::min<int64_t>(items, device_cus())), dim3(256), 0, st, p);
+      return;
   }
 }
 
@@ -403,6 +729,7 @@ extern "C" int lx2v_gemm_fp8_block128(const uint8_t* A, int64_t lda, const float
   p.per = q.per;
   p.tiles_m = (int)((M + q.tm - 1) / q.tm);
   p.tiles_n = (int)((N + q.tn - 1) / q.tn);
+  p.group_rcp = (uint32_t)((1ULL << 32) / (uint64_t)(GROUP_M * p.tiles_n));
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.split, joins = (M * N / 4 + 255) / 256;
   LX2V_REQUIRE(items < (1LL << 31) && (p.split == 1 || joins < (1LL << 31)), LX2V_EUNSUP, "gemm_fp8_block128: too many tiles");
   hipStream_t st = (hipStream_t)stream;

@@ -7,8 +7,8 @@ then do silently break results:
   * touch the VGPR destination of an inline-asm MFMA (a copy when it splits a live range, say) before
     the MFMA has written it -- an error when a compiler-generated instruction reads or writes such
     registers before any further MFMA has been issued (the next MFMA issues when the pipe is free,
-    which is when the first one has finished its passes), counted as a note when one MFMA lies
-    between.  MFMAs the compiler emitted itself (builtins) are its own business: it knows their latency;
+    which is when the first one has finished its passes) and before 20 wait states of inline-asm s_nop,
+    counted as a note when one MFMA lies between.  MFMAs the compiler emitted itself (builtins) are its own business: it knows their latency;
   * move data through the ring registers -- flagged for any compiler-generated instruction that
     names a register at or above --ring-base;
   * touch the VGPR destination of an inline-asm LDS read before a wait: the read returns at once and
@@ -56,7 +56,12 @@ def check(path, kernel_filter, ring_base):
         pending = []  # [regs, mfmas_seen, text]
         landing = []  # [regs, text] of asm LDS reads into VGPRs that no wait has covered yet
         notes = 0
+        nops = 0
         for t, from_asm in rows:
+            # wait states the author wrote behind the last MFMA: 20 are more than any of these instructions takes to write its result
+            nops = nops + int(t.split()[1]) + 1 if from_asm and t.startswith("s_nop") else 0
+            if nops >= 20:
+                pending = []
             if t.startswith("s_waitcnt") and "lgkmcnt" in t:
                 landing = []
             if not from_asm:
