@@ -113,6 +113,9 @@ LX2V_DEVICE void finish4(const Params& p, const f32x4& acc, int64_t m, int n) {
 // Workgroup = 4 waves (2 x 2), wave tile 16 MT x 16 NT, a ring of S operand tiles in LDS.  Slot: A rows | W rows (128
 // bytes a row, 16-byte chunk c at position c ^ ((row >> 1) & 7)) | 1 KiB of scales (256 bytes filled by each wave's one
 // 4-byte DMA: waves 0 .. the A scales of 64 rows each, wave 3 the weight scales of the tile's one or two row blocks).
+// A lane's 32 bytes of K are chunks fq and fq + 4 of its row, not two adjacent ones: any split of the 128 bytes serves as long as
+// both operands use the same one, and a ds_read_b128 serves lanes 0-3, 12-15, 20-27 (and so on) together, which with this
+// split fall on different banks and with adjacent chunks on the same ones two by two.
 template <int MT, int NT, int S>
 struct Tile {
   static constexpr int TM = 32 * MT, TN = 32 * NT;
@@ -176,13 +179,13 @@ __global__ __launch_bounds__(256) void gemm_fp8_block_tile_kernel(const Params p
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(slot + T::A_BYTES + T::W_BYTES + 256 * wid)), "v"(s_pv), "s"(s_rs) : "memory");
   };
 
-  int rd_a[2], rd_w[2];  // the lane's 32 bytes of K: chunks 2 fq, 2 fq + 1 of its row; 16 rows on: + 2048 bytes
+  int rd_a[2], rd_w[2];  // the lane's 32 bytes of K: chunks fq and fq + 4 of its row (see Tile); 16 rows on: + 2048 bytes
   {
     const int ar = wm * 16 * MT + fr, wr = wn * 16 * NT + fr;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      rd_a[c] = ar * BK + (((2 * fq + c) ^ ((ar >> 1) & 7)) << 4);
-      rd_w[c] = T::A_BYTES + wr * BK + (((2 * fq + c) ^ ((wr >> 1) & 7)) << 4);
+      rd_a[c] = ar * BK + (((fq + 4 * c) ^ ((ar >> 1) & 7)) << 4);
+      rd_w[c] = T::A_BYTES + wr * BK + (((fq + 4 * c) ^ ((wr >> 1) & 7)) << 4);
     }
   }
   auto frag = [&](const char* base, const int (&rd)[2], int i) __attribute__((always_inline)) -> i32x8 {
@@ -359,22 +362,30 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     s_step_hi = __builtin_amdgcn_readfirstlane((uint32_t)(step >> 32));
   }
   uint32_t dma_base = lds_base + 1024 * (uint32_t)wid, dma_sc = lds_base + 256 * (uint32_t)wid;
-  auto dma16 = [&](auto dstc, const u32x4& rs, int voff, uint32_t soff) __attribute__((always_inline)) {  // (the immediate in the M0 write: no register per target)
-    const uint32_t base = dma_base;
-    asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(base), "v"(voff), "s"(rs), "s"(soff), "i"(decltype(dstc)::value) : "memory", "scc");
+  auto set_m0 = [&](uint32_t base, auto ofsc) __attribute__((always_inline)) { asm volatile("s_add_u32 m0, %0, %1" ::"s"(base), "i"(decltype(ofsc)::value) : "memory", "scc"); };
+  auto load16 = [&](const u32x4& rs, int voff, uint32_t soff) __attribute__((always_inline)) {
+    asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(rs), "s"(soff) : "memory");
   };
-  auto dma4 = [&](auto dstc, const u32x4& rs, int voff) __attribute__((always_inline)) {
-    const uint32_t base = dma_sc;
-    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(base), "v"(voff), "s"(rs), "i"(decltype(dstc)::value) : "memory", "scc");
-  };
+  auto load4 = [&](const u32x4& rs, int voff) __attribute__((always_inline)) { asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rs) : "memory"); };
   const int a_step = 32 * (int)p.lda, w_step = 32 * (int)p.ldw;
-  auto dma = [&](auto Pc, auto qc) __attribute__((always_inline)) {  // piece q of the cursor's block into slot P: the weight's, the activation's, the scales
+  // piece q of the cursor's block into slot P (the weight's, the activation's, the scales): target and offset, then the load itself
+  int d_voff = 0;
+  auto dma_set = [&](auto Pc, auto qc) __attribute__((always_inline)) {
     constexpr int P = decltype(Pc)::value, q = decltype(qc)::value;
-    if constexpr (q < T::PW) dma16(IntC<T::W_AT + P * T::W_BYTES + 4096 * q>{}, w_rs, w_pv + q * w_step, d_soff);
-    else if constexpr (q < T::PW + T::PA) dma16(IntC<P * T::A_BYTES + 4096 * (q - T::PW)>{}, a_rs, a_pv + (q - T::PW) * a_step, d_soff);
-    else dma4(IntC<T::S_AT + P * 1024>{}, s_rs, s_pv);
+    if constexpr (q < T::PW) set_m0(dma_base, IntC<T::W_AT + P * T::W_BYTES + 4096 * q>{});
+    else if constexpr (q < T::PW + T::PA) set_m0(dma_base, IntC<P * T::A_BYTES + 4096 * (q - T::PW)>{});
+    else set_m0(dma_sc, IntC<T::S_AT + P * 1024>{});
+    d_voff = q == 0 ? w_pv : q < T::PW ? d_voff + w_step : q == T::PW ? a_pv : d_voff + a_step;
+    asm volatile("" : "+v"(d_voff));
+  };
+  auto dma_go = [&](auto qc) __attribute__((always_inline)) {
+    constexpr int q = decltype(qc)::value;
+    if constexpr (q < T::PW) load16(w_rs, d_voff, d_soff);
+    else if constexpr (q < T::PW + T::PA) load16(a_rs, d_voff, d_soff);
+    else load4(s_rs, s_pv);
   };
   constexpr int PIECES = T::PW + T::PA + 1;
+  static_assert(2 * PIECES <= T::STEPS, "a piece takes two steps");
   auto d_advance = [&]() __attribute__((always_inline)) {
     const uint32_t lo = s_rs[0] + s_step_lo;
     s_rs[1] += s_step_hi + (lo < s_step_lo ? 1u : 0u);
@@ -400,8 +411,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     const int ar = wm * 16 * MT + fr, wr = wn * 128 + fr;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      rd_a[c] = (int)lds_base + ar * BK + (((2 * fq + c) ^ ((ar >> 1) & 7)) << 4);
-      rd_w[c] = (int)lds_base + T::W_AT + wr * BK + (((2 * fq + c) ^ ((wr >> 1) & 7)) << 4);
+      rd_a[c] = (int)lds_base + ar * BK + (((fq + 4 * c) ^ ((ar >> 1) & 7)) << 4);
+      rd_w[c] = (int)lds_base + T::W_AT + wr * BK + (((fq + 4 * c) ^ ((wr >> 1) & 7)) << 4);
     }
   }
   const char* rd_s = lds + T::S_AT + (wm * 16 * MT + fr) * 4;
@@ -450,12 +461,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     static_for<0, T::STEPS>([&](auto tc) __attribute__((always_inline)) {
       constexpr int t = decltype(tc)::value;
       mm(part[t % 3], part[(t + 1) % 3], IntC<FRAG0 + P * SET + 8 * (t % 8)>{}, IntC<FRAG0 + P * SET + 64 + 8 * (t / 8)>{});
+      // Behind the MFMA its shadow of 32 cycles is filled with the four additions (16) and at most three more instructions: a
+      // piece's target and offset with an LDS read in an even step, its load in the next one; the other reads follow, spread out.
+      if constexpr (t < 2 * PIECES) {
+        if constexpr (t % 2 == 0) dma_set(IntC<P>{}, IntC<t / 2>{});
+        else dma_go(IntC<t / 2>{});
+      }
+      if constexpr (t < 2 * PIECES && t % 2 == 0) rd(IntC<Q>{}, IntC<t / 2>{});
+      if constexpr (t >= 2 * PIECES) {
+        constexpr int n = READS - PIECES, u = t - 2 * PIECES, steps = T::STEPS - 2 * PIECES - 1;
+        if constexpr (u < steps)
+          static_for<PIECES + u * n / steps, PIECES + (u + 1) * n / steps>([&](auto rc) __attribute__((always_inline)) { rd(IntC<Q>{}, rc); });
+      }
+      __builtin_amdgcn_sched_barrier(0);
       if constexpr (t >= 2) add(IntC<t - 2>{}, s[(t - 2) / 8]);
       else add(IntC<T::STEPS - 2 + t>{}, s_last);  // the previous block's last two
-      if constexpr (t < PIECES) dma(IntC<P>{}, IntC<t>{});
-      static_for<t * READS / (T::STEPS - 4), (t + 1) * READS / (T::STEPS - 4)>([&](auto rc) __attribute__((always_inline)) {
-        if constexpr (decltype(rc)::value < READS) rd(IntC<Q>{}, rc);
-      });
       __builtin_amdgcn_sched_barrier(0);
     });
     d_advance();
@@ -522,10 +542,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   };
 
   // ---- prologue: blocks 0 and 1 staged, fragments of block 0 ----
-  static_for<0, PIECES>([&](auto qc) __attribute__((always_inline)) { dma(IntC<0>{}, qc); });
-  d_advance();
-  static_for<0, PIECES>([&](auto qc) __attribute__((always_inline)) { dma(IntC<1>{}, qc); });
-  d_advance();
+  static_for<0, 2>([&](auto Pc) __attribute__((always_inline)) {
+    static_for<0, PIECES>([&](auto qc) __attribute__((always_inline)) {
+      dma_set(Pc, qc);
+      asm volatile("s_nop 0");
+      dma_go(qc);
+    });
+    d_advance();
+  });
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
