@@ -245,19 +245,21 @@ __global__ __launch_bounds__(256) void gemm_fp8_block_tile_kernel(const Params p
 
 // ---- stream kernel ------------------------------------------------------------------------------------
 // Long products: one wave per SIMD, 4 waves (2 x 2), wave tile 16 MT x 128 (one row block of weight scales), persistent: a
-// workgroup walks its output tiles as one stream of K blocks.  Three stages: block j + 2 is on its way into LDS, block
-// j + 1 is read from LDS into fragment registers, block j is multiplied -- fragments are double-buffered in registers, so
-// the LDS reads are spread over the whole block and only two LDS slots are needed.
-// LDS: A slot 0, 1 | W slot 0, 1 | scales 0, 1.
+// workgroup walks its output tiles as one stream of K blocks.  Block j is multiplied while block j + 1 is read from LDS into
+// the other set of fragment registers (so the LDS reads are spread over the whole block) and the blocks behind it are on
+// their way: once every wave has block j in registers, its slots take W(j + 2) and its scales, issued first, which have one
+// block's time to arrive, and A(j + 3), which has two.  LDS: three A slots, two W slots, two of scales.
 template <int MT>
 struct Stream {
   static constexpr int TM = 32 * MT, TN = 256;
   static constexpr int A_BYTES = TM * BK, W_BYTES = TN * BK;
-  static constexpr int W_AT = 2 * A_BYTES, S_AT = W_AT + 2 * W_BYTES;
+  static constexpr int W_AT = 3 * A_BYTES, S_AT = W_AT + 2 * W_BYTES;
   static constexpr int LDS = S_AT + 2 * 1024;
-  static constexpr int PA = TM / 32, PW = TN / 32;
+  static constexpr int PA = TM / 32, PW = TN / 32;  // DMA pieces of 1 KiB a wave
+  static constexpr int PIECES = PW + 1 + PA;        // W(j + 2), its scales, A(j + 3)
   static constexpr int STEPS = 8 * MT;
   static_assert(STEPS % 3 == 0, "the ring of three results wraps with the block");
+  static_assert(2 * PIECES <= STEPS, "a piece takes two steps");
   static constexpr int STORES = 4 * MT;
 };
 
@@ -326,40 +328,50 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   constexpr int NOWHERE = (int)0x80000000u;
   const bool sw_wave = wid == 3, sa_wave = wid < (T::TM + 63) / 64;
 
-  // ---- DMA cursor: two blocks ahead of the multiplied one ----
+  // ---- DMA cursors: W and its scales two blocks ahead of the multiplied one, A three ----
   // piece q of wave w: rows 32 q + 8 w + (lane >> 3) of the operand tile; the swizzle is the same for all q
   const int chunk = (lane & 7) ^ ((4 * wid + (lane >> 4)) & 7);
   const int left = p.K - (nk - 1) * BK;  // columns of the last block
-  int a_pv, w_pv;
-  auto set_voff = [&](bool last) __attribute__((always_inline)) {
-    const int r = 8 * wid + (lane >> 3);
-    const bool out = last && chunk * 16 >= left;
-    a_pv = out ? NOWHERE : r * (int)p.lda + chunk * 16;
-    w_pv = out ? NOWHERE : r * (int)p.ldw + chunk * 16;
+  const int ragged = left < BK ? nk - 1 : -1;
+  int a_pv, w_pv, s_pv = NOWHERE;
+  auto offset = [&](int64_t ld, bool last) __attribute__((always_inline)) -> int {  // of piece 0; `last`: chunks past K go nowhere
+    return last && chunk * 16 >= left ? NOWHERE : (8 * wid + (lane >> 3)) * (int)ld + chunk * 16;
   };
-  set_voff(nk == 1);
-  int d_ord = 0, d_kt = 0, s_pv = NOWHERE;
-  uint32_t d_soff = 0;
+  struct Cursor {
+    int ord = 0, kt = 0;
+    uint32_t soff = 0;
+  } ca, cw;
   u32x4 a_rs, w_rs, s_rs;
-  uint32_t s_step_lo = 0, s_step_hi = 0;  // bytes from the scales of one block to the next
-  auto d_tile = [&]() __attribute__((always_inline)) {  // descriptors of the cursor's output tile; past the last one they are empty
+  // the scales' descriptor moves on by a block's scales: 64-bit base, the same extent
+  uint64_t s_base = 0, s_step = 0;
+  auto a_tile = [&]() __attribute__((always_inline)) {  // descriptor of the cursor's output tile; past the last one it is empty
     const ParamsAgain p = params_again();
-    const int vbid = d_ord * grid + (int)blockIdx.x;
+    const int vbid = ca.ord * grid + (int)blockIdx.x;
     const bool live = vbid < ntiles;
     int m0 = 0, n0 = 0;
     if (live) tile_origin(p, vbid, T::TM, T::TN, m0, n0);
     a_rs = raw_descriptor(p->A + (int64_t)m0 * p->lda, live ? min((int64_t)p->M - m0, (int64_t)T::TM) * p->lda : 0);
+  };
+  auto w_tile = [&]() __attribute__((always_inline)) {
+    const ParamsAgain p = params_again();
+    const int vbid = cw.ord * grid + (int)blockIdx.x;
+    const bool live = vbid < ntiles;
+    int m0 = 0, n0 = 0;
+    if (live) tile_origin(p, vbid, T::TM, T::TN, m0, n0);
     w_rs = raw_descriptor(p->W + (int64_t)n0 * p->ldw, live ? min((int64_t)p->N - n0, (int64_t)T::TN) * p->ldw : 0);
     const int nb = min(((p->N + 127) >> 7) - (n0 >> 7), 2);
     const float* sb = sw_wave ? p->w_scale + (int64_t)(n0 >> 7) * p->lds_w : p->a_scale + m0;
     s_rs = raw_descriptor(sb, !live ? 0 : sw_wave ? ((int64_t)(nb - 1) * p->lds_w + 1) * 4 : sa_wave ? ((int64_t)p->M - m0) * 4 : 0);
+    s_base = ((uint64_t)s_rs[1] << 32) | s_rs[0];
     s_pv = sw_wave ? (lane < nb ? lane * (int)p->lds_w * 4 : NOWHERE) : (64 * wid + lane) * 4;
   };
-  d_tile();
+  a_tile();
+  w_tile();
+  a_pv = offset(p.lda, nk == 1);
+  w_pv = offset(p.ldw, nk == 1);
   {
     const int64_t step = sw_wave ? 4 : p.lds_a * 4;
-    s_step_lo = __builtin_amdgcn_readfirstlane((uint32_t)step);
-    s_step_hi = __builtin_amdgcn_readfirstlane((uint32_t)(step >> 32));
+    s_step = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)step >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)step);
   }
   uint32_t dma_base = lds_base + 1024 * (uint32_t)wid, dma_sc = lds_base + 256 * (uint32_t)wid;
   auto set_m0 = [&](uint32_t base, auto ofsc) __attribute__((always_inline)) { asm volatile("s_add_u32 m0, %0, %1" ::"s"(base), "i"(decltype(ofsc)::value) : "memory", "scc"); };
@@ -367,56 +379,76 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(rs), "s"(soff) : "memory");
   };
   auto load4 = [&](const u32x4& rs, int voff) __attribute__((always_inline)) { asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rs) : "memory"); };
-  const int a_step = 32 * (int)p.lda, w_step = 32 * (int)p.ldw;
-  // piece q of the cursor's block into slot P (the weight's, the activation's, the scales): target and offset, then the load itself
-  int d_voff = 0;
+  // piece q of a block's DMA, its target and then the load itself: W(j + 2), its scales, both into slot P, and A(j + 3) into the A slot at a_cur
+  uint32_t a_cur = dma_base, a_nxt = dma_base + T::A_BYTES;
   auto dma_set = [&](auto Pc, auto qc) __attribute__((always_inline)) {
     constexpr int P = decltype(Pc)::value, q = decltype(qc)::value;
     if constexpr (q < T::PW) set_m0(dma_base, IntC<T::W_AT + P * T::W_BYTES + 4096 * q>{});
-    else if constexpr (q < T::PW + T::PA) set_m0(dma_base, IntC<P * T::A_BYTES + 4096 * (q - T::PW)>{});
-    else set_m0(dma_sc, IntC<T::S_AT + P * 1024>{});
-    d_voff = q == 0 ? w_pv : q < T::PW ? d_voff + w_step : q == T::PW ? a_pv : d_voff + a_step;
-    asm volatile("" : "+v"(d_voff));
+    else if constexpr (q == T::PW) set_m0(dma_sc, IntC<T::S_AT + P * 1024>{});
+    else set_m0(a_cur, IntC<4096 * (q - T::PW - 1)>{});
   };
+  const int a_step = 32 * (int)p.lda, w_step = 32 * (int)p.ldw;
+  int d_voff = 0;
   auto dma_go = [&](auto qc) __attribute__((always_inline)) {
     constexpr int q = decltype(qc)::value;
-    if constexpr (q < T::PW) load16(w_rs, d_voff, d_soff);
-    else if constexpr (q < T::PW + T::PA) load16(a_rs, d_voff, d_soff);
-    else load4(s_rs, s_pv);
+    if constexpr (q == 0) d_voff = w_pv;
+    if constexpr (q < T::PW) {
+      load16(w_rs, d_voff, cw.soff);
+      if constexpr (q + 1 < T::PW) d_voff += w_step;
+    } else if constexpr (q == T::PW) {
+      load4(s_rs, s_pv);
+    } else {
+      if constexpr (q == T::PW + 1) d_voff = a_pv;
+      load16(a_rs, d_voff, ca.soff);
+      if constexpr (q + 1 < T::PIECES) d_voff += a_step;
+    }
+    asm volatile("" : "+v"(d_voff));
   };
-  constexpr int PIECES = T::PW + T::PA + 1;
-  static_assert(2 * PIECES <= T::STEPS, "a piece takes two steps");
-  auto d_advance = [&]() __attribute__((always_inline)) {
-    const uint32_t lo = s_rs[0] + s_step_lo;
-    s_rs[1] += s_step_hi + (lo < s_step_lo ? 1u : 0u);
-    s_rs[0] = lo;
-    ++d_kt;
-    d_soff += BK;
-    if (d_kt == nk - 1) {
-      if (left < BK) set_voff(true);
+  auto w_advance = [&]() __attribute__((always_inline)) {
+    ++cw.kt;
+    cw.soff += BK;
+    s_base += s_step;
+    s_rs[0] = (uint32_t)s_base;
+    s_rs[1] = (uint32_t)(s_base >> 32);
+    if (cw.kt == ragged) w_pv = offset(params_again()->ldw, true);
+    if (cw.kt == nk) {
+      cw.kt = 0;
+      cw.soff = 0;
+      ++cw.ord;
+      w_tile();
+      if (ragged >= 0) w_pv = offset(params_again()->ldw, nk == 1);
     }
-    if (d_kt == nk) {
-      if (left < BK) set_voff(nk == 1);
-      d_kt = 0;
-      d_soff = 0;
-      ++d_ord;
-      d_tile();
+    asm volatile("" : "+s"(w_rs), "+s"(s_rs), "+s"(cw.soff), "+s"(dma_base), "+s"(dma_sc));
+  };
+  auto a_advance = [&]() __attribute__((always_inline)) {
+    ++ca.kt;
+    ca.soff += BK;
+    if (ca.kt == ragged) a_pv = offset(params_again()->lda, true);
+    if (ca.kt == nk) {
+      ca.kt = 0;
+      ca.soff = 0;
+      ++ca.ord;
+      a_tile();
+      if (ragged >= 0) a_pv = offset(params_again()->lda, nk == 1);
     }
-    asm volatile("" : "+s"(a_rs), "+s"(w_rs), "+s"(s_rs), "+s"(dma_base), "+s"(dma_sc));
+    a_cur = a_nxt;
+    a_nxt = a_nxt == dma_base + 2 * T::A_BYTES ? dma_base : a_nxt + T::A_BYTES;
+    asm volatile("" : "+s"(a_rs), "+s"(ca.soff), "+s"(a_cur), "+s"(a_nxt));
   };
 
   // ---- fragments: register set P (0 | 1) = 8 W fragments, then MT A fragments, of 8 accumulator registers each ----
-  int rd_a[2], rd_w[2];  // LDS addresses of the lane's two 16-byte halves at row block 0
+  int rd_a[2], rd_w[2];  // LDS addresses of the lane's two 16-byte halves at row block 0 of slot 0 (A: less this wave's share of the DMA target)
   {
     const int ar = wm * 16 * MT + fr, wr = wn * 128 + fr;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      rd_a[c] = (int)lds_base + ar * BK + (((fq + 4 * c) ^ ((ar >> 1) & 7)) << 4);
+      rd_a[c] = ar * BK + (((fq + 4 * c) ^ ((ar >> 1) & 7)) << 4) - 1024 * wid;
       rd_w[c] = (int)lds_base + T::W_AT + wr * BK + (((fq + 4 * c) ^ ((wr >> 1) & 7)) << 4);
     }
   }
   const char* rd_s = lds + T::S_AT + (wm * 16 * MT + fr) * 4;
   const char* rd_sw = lds + T::S_AT + 768 + wn * 4;
+  int at_a[2];  // rd_a in the slot being read
   constexpr int FRAG0 = 32, SET = 8 * (8 + MT);
   static_assert(FRAG0 + 2 * SET <= 256, "fragments exceed the accumulator registers");
   float sa[MT], sw, s[MT], s_last;
@@ -437,24 +469,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   auto lds_frag = [&](int addr, auto dstc, auto ofsc) __attribute__((always_inline)) {  // 16 bytes a lane into four accumulator registers; waited for at the next barrier
     asm volatile("ds_read_b128 a[%1:%2], %0 offset:%3" ::"v"(addr), "n"(decltype(dstc)::value), "n"(decltype(dstc)::value + 3), "n"(decltype(ofsc)::value) : "memory", FRAG_CLOBBERS);
   };
-  // LDS read r of a block from slot P into register set P: 16 halves of W, 2 MT of A, MT + 1 scales
+  // LDS read r of a block into register set P: 16 halves of W, 2 MT of A, MT + 1 scales
   auto rd = [&](auto Pc, auto rc) __attribute__((always_inline)) {
     constexpr int P = decltype(Pc)::value, r = decltype(rc)::value;
     if constexpr (r < 16) lds_frag(rd_w[r & 1], IntC<FRAG0 + P * SET + 4 * r>{}, IntC<P * T::W_BYTES + (r >> 1) * 2048>{});
-    else if constexpr (r < 16 + 2 * MT) lds_frag(rd_a[r & 1], IntC<FRAG0 + P * SET + 4 * r>{}, IntC<P * T::A_BYTES + ((r - 16) >> 1) * 2048>{});
+    else if constexpr (r < 16 + 2 * MT) lds_frag(at_a[r & 1], IntC<FRAG0 + P * SET + 4 * r>{}, IntC<((r - 16) >> 1) * 2048>{});
     else if constexpr (r < 16 + 3 * MT) sa[r - 16 - 2 * MT] = *reinterpret_cast<const float*>(rd_s + P * 1024 + (r - 16 - 2 * MT) * 64);
     else if constexpr (r == 16 + 3 * MT) sw = *reinterpret_cast<const float*>(rd_sw + P * 1024);
   };
   constexpr int READS = 17 + 3 * MT;
 
-  // One block: multiply register set P, read the next one's fragments from slot 1 - P, stage the one after into slot P.
+  // One block: multiply register set P, read the next one's fragments into set 1 - P, stage into the slots of this one.
   auto block = [&](auto Pc, bool relaxed) __attribute__((always_inline)) {
     constexpr int P = decltype(Pc)::value, Q = 1 - P;
     // the next block is complete in LDS once every wave is past this barrier, and every wave has read its fragments of this one
-    if (relaxed) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::STORES) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    // (what was issued behind the next block's last pieces may still be on its way: the pieces of the block after it, an epilogue's stores)
+    if (relaxed) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::PA + T::STORES) : "memory");
+    else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::PA) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+    at_a[0] = rd_a[0] + (int)a_nxt;
+    at_a[1] = rd_a[1] + (int)a_nxt;
     s_last = s[MT - 1];
 #pragma unroll
     for (int i = 0; i < MT; ++i) s[i] = sa[i] * sw;
@@ -462,23 +497,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       constexpr int t = decltype(tc)::value;
       mm(part[t % 3], part[(t + 1) % 3], IntC<FRAG0 + P * SET + 8 * (t % 8)>{}, IntC<FRAG0 + P * SET + 64 + 8 * (t / 8)>{});
       // Behind the MFMA its shadow of 32 cycles is filled with the four additions (16) and at most three more instructions: a
-      // piece's target and offset with an LDS read in an even step, its load in the next one; the other reads follow, spread out.
-      if constexpr (t < 2 * PIECES) {
+      // piece's target with two LDS reads in an even step, its load in the next one; the reads left follow, two a step, early enough
+      // to be complete at the block's end.
+      if constexpr (t < 2 * T::PIECES) {
         if constexpr (t % 2 == 0) dma_set(IntC<P>{}, IntC<t / 2>{});
         else dma_go(IntC<t / 2>{});
       }
-      if constexpr (t < 2 * PIECES && t % 2 == 0) rd(IntC<Q>{}, IntC<t / 2>{});
-      if constexpr (t >= 2 * PIECES) {
-        constexpr int n = READS - PIECES, u = t - 2 * PIECES, steps = T::STEPS - 2 * PIECES - 1;
-        if constexpr (u < steps)
-          static_for<PIECES + u * n / steps, PIECES + (u + 1) * n / steps>([&](auto rc) __attribute__((always_inline)) { rd(IntC<Q>{}, rc); });
+      if constexpr (t % 2 == 0 || t >= 2 * T::PIECES) {
+        constexpr int r = t < 2 * T::PIECES ? t : 2 * t - 2 * T::PIECES;
+        if constexpr (r < READS) rd(IntC<Q>{}, IntC<r>{});
+        if constexpr (r + 1 < READS) rd(IntC<Q>{}, IntC<r + 1>{});
       }
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (t >= 2) add(IntC<t - 2>{}, s[(t - 2) / 8]);
       else add(IntC<T::STEPS - 2 + t>{}, s_last);  // the previous block's last two
       __builtin_amdgcn_sched_barrier(0);
     });
-    d_advance();
+    w_advance();
+    a_advance();
   };
 
   // ---- epilogue: a lane's four columns become eight consecutive ones by swapping lane rows between two column blocks;
@@ -541,15 +577,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     }
   };
 
-  // ---- prologue: blocks 0 and 1 staged, fragments of block 0 ----
-  static_for<0, 2>([&](auto Pc) __attribute__((always_inline)) {
-    static_for<0, PIECES>([&](auto qc) __attribute__((always_inline)) {
-      dma_set(Pc, qc);
-      asm volatile("s_nop 0");
-      dma_go(qc);
-    });
-    d_advance();
+  // ---- prologue: W(0), W(1) and their scales, A(0), A(1), A(2), then the fragments of block 0 ----
+  auto piece = [&](auto Pc, auto qc) __attribute__((always_inline)) {
+    dma_set(Pc, qc);
+    asm volatile("s_nop 0");
+    dma_go(qc);
+  };
+  static_for<0, 3>([&](auto bc) __attribute__((always_inline)) {
+    constexpr int b = decltype(bc)::value;
+    if constexpr (b < 2) {
+      static_for<0, T::PW + 1>([&](auto qc) __attribute__((always_inline)) { piece(bc, qc); });
+      w_advance();
+    }
+    static_for<T::PW + 1, T::PIECES>([&](auto qc) __attribute__((always_inline)) { piece(IntC<0>{}, qc); });
+    a_advance();
   });
+  // (the ring is back at slot 0: block 0's)
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -557,6 +600,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+  at_a[0] = rd_a[0] + (int)a_cur;
+  at_a[1] = rd_a[1] + (int)a_cur;
   static_for<0, READS>([&](auto rc) __attribute__((always_inline)) { rd(IntC<0>{}, rc); });
 #pragma unroll
   for (int i = 0; i < 3; ++i) part[i] = f32x4{0.f, 0.f, 0.f, 0.f};
