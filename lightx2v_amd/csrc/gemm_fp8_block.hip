@@ -273,14 +273,19 @@ LX2V_DEVICE void divmod(uint32_t n, uint32_t d, uint32_t rcp, uint32_t& q, uint3
   }
 }
 
-template <class P>
-LX2V_DEVICE void tile_origin(P p, int vbid, int tm, int tn, int& m0, int& n0) {
-  const uint32_t t = (uint32_t)xcd_remap(vbid, p->tiles_m * p->tiles_n);
-  uint32_t g, in_g, row, col;
-  divmod(t, (uint32_t)(GROUP_M * p->tiles_n), p->group_rcp, g, in_g);
-  const uint32_t gm = (uint32_t)min(p->tiles_m - (int)g * GROUP_M, GROUP_M);
+// Output tile -> its position: contiguous runs of tiles for each XCD, GROUP_M row panels sharing one sweep over the columns.
+struct Raster {
+  int tiles_m, tiles_n, per_xcd, extra;  // tiles / 8, tiles % 8
+  uint32_t rcp;                          // of GROUP_M * tiles_n
+};
+LX2V_DEVICE void tile_origin(const Raster& g, int vbid, int tm, int tn, int& m0, int& n0) {
+  const int xcd = vbid & 7;
+  const uint32_t t = (uint32_t)(xcd * g.per_xcd + min(xcd, g.extra) + (vbid >> 3));
+  uint32_t sweep, in_g, row, col;
+  divmod(t, (uint32_t)(GROUP_M * g.tiles_n), g.rcp, sweep, in_g);
+  const uint32_t gm = (uint32_t)min(g.tiles_m - (int)sweep * GROUP_M, GROUP_M);
   divmod(in_g, gm, gm == 4 ? 0x40000000u : gm == 3 ? 0x55555555u : gm == 2 ? 0x80000000u : 0xffffffffu, col, row);
-  m0 = (int)(g * GROUP_M + row) * tm;
+  m0 = (int)(sweep * GROUP_M + row) * tm;
   n0 = (int)col * tn;
 }
 
@@ -324,6 +329,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   const int64_t total = (int64_t)my_tiles * nk;
   if (total == 0) return;
 
+  const Raster raster{p.tiles_m, p.tiles_n, ntiles >> 3, ntiles & 7, p.group_rcp};
   const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t)(size_t)(__attribute__((address_space(3))) char*)lds);
   constexpr int NOWHERE = (int)0x80000000u;
   const bool sw_wave = wid == 3, sa_wave = wid < (T::TM + 63) / 64;
@@ -344,26 +350,37 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   u32x4 a_rs, w_rs, s_rs;
   // the scales' descriptor moves on by a block's scales: 64-bit base, the same extent
   uint64_t s_base = 0, s_step = 0;
+  // (the fields are read together: one wait for memory per tile and operand, not one for each field on its first use)
   auto a_tile = [&]() __attribute__((always_inline)) {  // descriptor of the cursor's output tile; past the last one it is empty
     const ParamsAgain p = params_again();
+    const uint64_t base = reinterpret_cast<uint64_t>(p->A);
+    const int64_t lda = p->lda;
+    const int M = p->M;
+    asm volatile("" ::"s"(base), "s"(lda), "s"(M));
     const int vbid = ca.ord * grid + (int)blockIdx.x;
-    const bool live = vbid < ntiles;
-    int m0 = 0, n0 = 0;
-    if (live) tile_origin(p, vbid, T::TM, T::TN, m0, n0);
-    a_rs = raw_descriptor(p->A + (int64_t)m0 * p->lda, live ? min((int64_t)p->M - m0, (int64_t)T::TM) * p->lda : 0);
+    int m0, n0;
+    tile_origin(raster, vbid, T::TM, T::TN, m0, n0);
+    const int rows = vbid < ntiles ? min(M - m0, T::TM) : 0;
+    a_rs = raw_descriptor(reinterpret_cast<const uint8_t*>(base) + (int64_t)(rows ? m0 : 0) * lda, (int64_t)rows * lda);
   };
   auto w_tile = [&]() __attribute__((always_inline)) {
     const ParamsAgain p = params_again();
+    const uint64_t base = reinterpret_cast<uint64_t>(p->W), asb = reinterpret_cast<uint64_t>(p->a_scale), wsb = reinterpret_cast<uint64_t>(p->w_scale);
+    const int64_t ldw = p->ldw, lds_w = p->lds_w;
+    const int M = p->M, N = p->N;
+    asm volatile("" ::"s"(base), "s"(asb), "s"(wsb), "s"(ldw), "s"(lds_w), "s"(M), "s"(N));
     const int vbid = cw.ord * grid + (int)blockIdx.x;
     const bool live = vbid < ntiles;
-    int m0 = 0, n0 = 0;
-    if (live) tile_origin(p, vbid, T::TM, T::TN, m0, n0);
-    w_rs = raw_descriptor(p->W + (int64_t)n0 * p->ldw, live ? min((int64_t)p->N - n0, (int64_t)T::TN) * p->ldw : 0);
-    const int nb = min(((p->N + 127) >> 7) - (n0 >> 7), 2);
-    const float* sb = sw_wave ? p->w_scale + (int64_t)(n0 >> 7) * p->lds_w : p->a_scale + m0;
-    s_rs = raw_descriptor(sb, !live ? 0 : sw_wave ? ((int64_t)(nb - 1) * p->lds_w + 1) * 4 : sa_wave ? ((int64_t)p->M - m0) * 4 : 0);
+    int m0, n0;
+    tile_origin(raster, vbid, T::TM, T::TN, m0, n0);
+    if (!live) m0 = n0 = 0;
+    const int rows = live ? min(N - n0, T::TN) : 0;
+    w_rs = raw_descriptor(reinterpret_cast<const uint8_t*>(base) + (int64_t)n0 * ldw, (int64_t)rows * ldw);
+    const int nb = min(((N + 127) >> 7) - (n0 >> 7), 2);
+    const float* sb = sw_wave ? reinterpret_cast<const float*>(wsb) + (int64_t)(n0 >> 7) * lds_w : reinterpret_cast<const float*>(asb) + m0;
+    s_rs = raw_descriptor(sb, !live ? 0 : sw_wave ? ((int64_t)(nb - 1) * lds_w + 1) * 4 : sa_wave ? ((int64_t)M - m0) * 4 : 0);
     s_base = ((uint64_t)s_rs[1] << 32) | s_rs[0];
-    s_pv = sw_wave ? (lane < nb ? lane * (int)p->lds_w * 4 : NOWHERE) : (64 * wid + lane) * 4;
+    s_pv = sw_wave ? (lane < nb ? lane * (int)lds_w * 4 : NOWHERE) : (64 * wid + lane) * 4;
   };
   a_tile();
   w_tile();
@@ -418,7 +435,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       w_tile();
       if (ragged >= 0) w_pv = offset(params_again()->ldw, nk == 1);
     }
-    asm volatile("" : "+s"(w_rs), "+s"(s_rs), "+s"(cw.soff), "+s"(dma_base), "+s"(dma_sc));
+    asm volatile("" : "+s"(w_rs), "+s"(s_rs), "+s"(s_base), "+s"(cw.soff), "+s"(cw.kt), "+s"(cw.ord), "+s"(dma_base), "+s"(dma_sc));
   };
   auto a_advance = [&]() __attribute__((always_inline)) {
     ++ca.kt;
@@ -433,7 +450,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     }
     a_cur = a_nxt;
     a_nxt = a_nxt == dma_base + 2 * T::A_BYTES ? dma_base : a_nxt + T::A_BYTES;
-    asm volatile("" : "+s"(a_rs), "+s"(ca.soff), "+s"(a_cur), "+s"(a_nxt));
+    asm volatile("" : "+s"(a_rs), "+s"(ca.soff), "+s"(ca.kt), "+s"(ca.ord), "+s"(a_cur), "+s"(a_nxt));
   };
 
   // ---- fragments: register set P (0 | 1) = 8 W fragments, then MT A fragments, of 8 accumulator registers each ----
@@ -460,10 +477,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     asm volatile("v_mfma_f32_16x16x128_f8f6f4 %0, a[%2:%3], a[%4:%5], 0"
                  : "=&v"(d), "+v"(old) : "n"(decltype(wc)::value), "n"(decltype(wc)::value + 7), "n"(decltype(ac)::value), "n"(decltype(ac)::value + 7));
   };
-  auto add = [&](auto tc, float sc) __attribute__((always_inline)) {
+  auto add = [&](auto tc, float sc, auto FIRSTc) __attribute__((always_inline)) {  // FIRST: the output tile's first block sets the sums
     constexpr int t = decltype(tc)::value;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[t / 8][t % 8][e] = __builtin_fmaf(part[t % 3][e], sc, acc[t / 8][t % 8][e]);
+    for (int e = 0; e < 4; ++e) acc[t / 8][t % 8][e] = decltype(FIRSTc)::value ? part[t % 3][e] * sc : __builtin_fmaf(part[t % 3][e], sc, acc[t / 8][t % 8][e]);
     asm volatile("" : "+v"(acc[t / 8][t % 8]));  // (pinned here: without a use the sums would sink to the end of the block and keep every result alive)
   };
   auto lds_frag = [&](int addr, auto dstc, auto ofsc) __attribute__((always_inline)) {  // 16 bytes a lane into four accumulator registers; waited for at the next barrier
@@ -480,7 +497,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   constexpr int READS = 17 + 3 * MT;
 
   // One block: multiply register set P, read the next one's fragments into set 1 - P, stage into the slots of this one.
-  auto block = [&](auto Pc, bool relaxed) __attribute__((always_inline)) {
+  auto block = [&](auto Pc, auto FIRSTc, bool relaxed) __attribute__((always_inline)) {
     constexpr int P = decltype(Pc)::value, Q = 1 - P;
     // the next block is complete in LDS once every wave is past this barrier, and every wave has read its fragments of this one
     // (what was issued behind the next block's last pieces may still be on its way: the pieces of the block after it, an epilogue's stores)
@@ -509,72 +526,98 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
         if constexpr (r + 1 < READS) rd(IntC<Q>{}, IntC<r + 1>{});
       }
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (t >= 2) add(IntC<t - 2>{}, s[(t - 2) / 8]);
-      else add(IntC<T::STEPS - 2 + t>{}, s_last);  // the previous block's last two
+      constexpr int last = T::STEPS - 2 + t;
+      if constexpr (t >= 2) add(IntC<t - 2>{}, s[(t - 2) / 8], FIRSTc);
+      else if constexpr (decltype(FIRSTc)::value) acc[last / 8][last % 8] = f32x4{0.f, 0.f, 0.f, 0.f};
+      else add(IntC<last>{}, s_last, FIRSTc);  // the previous block's last two
       __builtin_amdgcn_sched_barrier(0);
     });
-    w_advance();
-    a_advance();
   };
 
   // ---- epilogue: a lane's four columns become eight consecutive ones by swapping lane rows between two column blocks;
   // 16-byte stores through a descriptor of the tile's rows: rows past M and columns past N are dropped ----
   auto epilogue = [&](int m0, int n0) __attribute__((always_inline)) {
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" : "+v"(part[0]), "+v"(part[1]), "+v"(part[2]));  // the last MFMAs were issued a few cycles ago
-    add(IntC<T::STEPS - 2>{}, s[MT - 1]);
-    add(IntC<T::STEPS - 1>{}, s[MT - 1]);
-#pragma unroll
-    for (int i = 0; i < 3; ++i) part[i] = f32x4{0.f, 0.f, 0.f, 0.f};  // the next block adds its predecessor's last two once more
+    add(IntC<T::STEPS - 2>{}, s[MT - 1], IntC<0>{});
+    add(IntC<T::STEPS - 1>{}, s[MT - 1], IntC<0>{});
     const ParamsAgain p = params_again();
+    const uint64_t c_at = reinterpret_cast<uint64_t>(p->C), bias_at = reinterpret_cast<uint64_t>(p->bias), gate_at = reinterpret_cast<uint64_t>(p->gate), resid_at = reinterpret_cast<uint64_t>(p->resid);
+    const int64_t ldc = p->ldc, ldr = p->ldr;
+    const int M = p->M, N = p->N;
+    asm volatile("" ::"s"(c_at), "s"(bias_at), "s"(gate_at), "s"(resid_at), "s"(ldc), "s"(ldr), "s"(M), "s"(N));
     int fr_ = fr, fq_ = fq;
     asm volatile("" : "+v"(fr_), "+v"(fq_));
-    const u32x4 c_d = raw_descriptor(p->C + (int64_t)m0 * p->ldc, (min((int64_t)p->M - m0, (int64_t)T::TM) - 1) * p->ldc * 2 + (int64_t)p->N * 2);
-    void* cb = reinterpret_cast<void*>(((uint64_t)c_d[1] << 32) | c_d[0]);
-    const __amdgpu_buffer_rsrc_t c_rs = __builtin_amdgcn_make_buffer_rsrc(cb, 0, (int)c_d[2], 0x00020000);
-#pragma unroll
-    for (int k = 0; k < 8; k += 2) {
-      f32x4 bv[2], gv[2];
+    auto resource = [](uint64_t at, int64_t bytes) __attribute__((always_inline)) {  // accesses past the end: loads give 0, stores are dropped
+      const u32x4 d = raw_descriptor(reinterpret_cast<const void*>(at), bytes);
+      return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)d[1] << 32) | d[0]), 0, (int)d[2], 0x00020000);
+    };
+    const int64_t rows = min(M - m0, T::TM);
+    const auto c_rs = resource(c_at + (int64_t)m0 * ldc * 2, (rows - 1) * ldc * 2 + (int64_t)N * 2);
+    const auto r_rs = resource(resid_at + (int64_t)m0 * ldr * 2, EPI == LX2V_EPI_RESIDUAL ? (rows - 1) * ldr * 2 + (int64_t)N * 2 : 0);
+    const auto b_rs = resource(bias_at, bias_at ? (int64_t)N * 4 : 0), g_rs = resource(gate_at, EPI == LX2V_EPI_RESIDUAL && gate_at ? (int64_t)N * 4 : 0);
+    // step u = column block pair u / MT, row block u % MT.  Bias and gate are loaded one pair ahead, residual rows RV steps ahead.
+    // (the residual form has registers for one pair's bias and gate only)
+    constexpr int U = 4 * MT, RV = 2, CV = EPI == LX2V_EPI_RESIDUAL ? 1 : 2;
+    const int col0 = n0 + wn * 128 + fq_ * 4;
+    f32x4 bv[CV][2], gv[CV][2];
+    u32x2 rv[RV][2];
+    auto fetch_cols = [&](auto kc) __attribute__((always_inline)) {
+      constexpr int k2 = decltype(kc)::value;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int n = min(n0 + wn * 128 + (k + h) * 16 + fq_ * 4, p->N - 4);
-        bv[h] = p->bias != nullptr ? *reinterpret_cast<const f32x4*>(p->bias + n) : f32x4{0.f, 0.f, 0.f, 0.f};
-        gv[h] = EPI == LX2V_EPI_RESIDUAL && p->gate != nullptr ? *reinterpret_cast<const f32x4*>(p->gate + n) : f32x4{1.f, 1.f, 1.f, 1.f};
-      }
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const int row = wm * 16 * MT + i * 16 + fr_;
-        uint32_t d[2][2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[e] = acc[i][k + h][e] + bv[h][e];
-            if constexpr (EPI == LX2V_EPI_GELU_TANH) v[e] = gelu_tanh(v[e]);
-            if constexpr (EPI == LX2V_EPI_RESIDUAL) v[e] *= gv[h][e];
-          }
-          if constexpr (EPI == LX2V_EPI_RESIDUAL) {
-            const int m = min(m0 + row, p->M - 1), n = min(n0 + wn * 128 + (k + h) * 16 + fq_ * 4, p->N - 4);
-            const u32x2 r = *reinterpret_cast<const u32x2*>(p->resid + (int64_t)m * p->ldr + n);
-            v[0] += __uint_as_float(r[0] << 16);
-            v[1] += __uint_as_float(r[0] & 0xffff0000u);
-            v[2] += __uint_as_float(r[1] << 16);
-            v[3] += __uint_as_float(r[1] & 0xffff0000u);
-          }
-          d[h][0] = pack2(v[0], v[1]);
-          d[h][1] = pack2(v[2], v[3]);
-          acc[i][k + h] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int at = (col0 + (2 * k2 + h) * 16) * 4;
+        bv[k2 % CV][h] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(b_rs, at, 0, 0));
+        if constexpr (EPI == LX2V_EPI_RESIDUAL) {
+          gv[k2 % CV][h] = f32x4{1.f, 1.f, 1.f, 1.f};
+          if (gate_at != 0) gv[k2 % CV][h] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(g_rs, at, 0, 0));
         }
-        // lane rows fq = 0 .. 3 of block k: columns 4 fq ..; swapping the odd rows of d[0] with the even rows of d[1] leaves row 0
-        // with columns 0-7 of block k, row 1 with 0-7 of block k + 1, row 2 with 8-15 of block k, row 3 with 8-15 of block k + 1
-        const auto x = __builtin_amdgcn_permlane16_swap(d[0][0], d[1][0], false, false);
-        const auto y = __builtin_amdgcn_permlane16_swap(d[0][1], d[1][1], false, false);
-        const int n = n0 + wn * 128 + (k + (fq_ & 1)) * 16 + (fq_ >> 1) * 8;
-        const bool in = m0 + row < p->M && n < p->N;
-        __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], y[0], x[1], y[1]}, c_rs, in ? (row * (int)p->ldc + n) * 2 : NOWHERE, 0, 0);
       }
+    };
+    auto fetch_rows = [&](auto uc) __attribute__((always_inline)) {
+      constexpr int u = decltype(uc)::value;
+      if constexpr (EPI == LX2V_EPI_RESIDUAL && u < U) {
+        const int at = ((wm * 16 * MT + (u % MT) * 16 + fr_) * (int)ldr + col0 + 2 * (u / MT) * 16) * 2;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) rv[u % RV][h] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r_rs, at + 32 * h, 0, 0));
+      }
+    };
+    fetch_cols(IntC<0>{});
+    static_for<0, RV>([&](auto uc) __attribute__((always_inline)) { fetch_rows(uc); });
+    static_for<0, U>([&](auto uc) __attribute__((always_inline)) {
+      constexpr int u = decltype(uc)::value, i = u % MT, k2 = u / MT, b = k2 % CV;
+      if constexpr (CV == 2 && i == 0 && k2 < 3) fetch_cols(IntC<k2 + 1>{});
+      const int row = wm * 16 * MT + i * 16 + fr_;
+      uint32_t d[2][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = acc[i][2 * k2 + h][e] + bv[b][h][e];
+          if constexpr (EPI == LX2V_EPI_GELU_TANH) v[e] = gelu_tanh(v[e]);
+        }
+        if constexpr (EPI == LX2V_EPI_RESIDUAL) {
+          const u32x2 r = rv[u % RV][h];
+          v[0] = v[0] * gv[b][h][0] + __uint_as_float(r[0] << 16);
+          v[1] = v[1] * gv[b][h][1] + __uint_as_float(r[0] & 0xffff0000u);
+          v[2] = v[2] * gv[b][h][2] + __uint_as_float(r[1] << 16);
+          v[3] = v[3] * gv[b][h][3] + __uint_as_float(r[1] & 0xffff0000u);
+        }
+        d[h][0] = pack2(v[0], v[1]);
+        d[h][1] = pack2(v[2], v[3]);
+      }
+      // lane rows fq = 0 .. 3 of block k: columns 4 fq ..; swapping the odd rows of d[0] with the even rows of d[1] leaves row 0
+      // with columns 0-7 of block k, row 1 with 0-7 of block k + 1, row 2 with 8-15 of block k, row 3 with 8-15 of block k + 1
+      const auto x = __builtin_amdgcn_permlane16_swap(d[0][0], d[1][0], false, false);
+      const auto y = __builtin_amdgcn_permlane16_swap(d[0][1], d[1][1], false, false);
+      const int n = n0 + wn * 128 + (2 * k2 + (fq_ & 1)) * 16 + (fq_ >> 1) * 8;
+      const bool in = m0 + row < M && n < N;
+      __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], y[0], x[1], y[1]}, c_rs, in ? (row * (int)ldc + n) * 2 : NOWHERE, 0, 0);
+      if constexpr (CV == 1 && i == MT - 1 && k2 < 3) fetch_cols(IntC<k2 + 1>{});
+      fetch_rows(IntC<u + RV>{});
+      asm volatile("" ::: FRAG_CLOBBERS);  // (the next block's fragments are in there: nothing of the epilogue may stay in them)
       __builtin_amdgcn_sched_barrier(0);
-    }
+    });
   };
 
   // ---- prologue: W(0), W(1) and their scales, A(0), A(1), A(2), then the fragments of block 0 ----
@@ -593,28 +636,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     a_advance();
   });
   // (the ring is back at slot 0: block 0's)
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) acc[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   at_a[0] = rd_a[0] + (int)a_cur;
   at_a[1] = rd_a[1] + (int)a_cur;
   static_for<0, READS>([&](auto rc) __attribute__((always_inline)) { rd(IntC<0>{}, rc); });
-#pragma unroll
-  for (int i = 0; i < 3; ++i) part[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < MT; ++i) s[i] = 0.f;
 
   int ord = 0, kt = 0;
   bool relaxed = false;
-  auto after = [&]() __attribute__((always_inline)) {
+  auto step = [&](auto Pc) __attribute__((always_inline)) {
+    if (kt == 0) block(Pc, IntC<1>{}, relaxed);
+    else block(Pc, IntC<0>{}, false);
+    w_advance();
+    a_advance();
     relaxed = false;
     if (++kt == nk) {
       int m0, n0;
-      tile_origin(params_again(), ord * grid + (int)blockIdx.x, T::TM, T::TN, m0, n0);
+      tile_origin(raster, ord * grid + (int)blockIdx.x, T::TM, T::TN, m0, n0);
       epilogue(m0, n0);
       relaxed = true;
       kt = 0;
@@ -622,12 +661,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     }
   };
   for (int64_t j = 0; j < total; j += 2) {
-    block(IntC<0>{}, relaxed);
-    after();
-    if (j + 1 < total) {
-      block(IntC<1>{}, relaxed);
-      after();
-    }
+    step(IntC<0>{});
+    if (j + 1 < total) step(IntC<1>{});
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA may still be writing this workgroup's LDS when it ends
 }
@@ -773,6 +808,7 @@ extern "C" int lx2v_gemm_fp8_block128(const uint8_t* A, int64_t lda, const float
   LX2V_REQUIRE(lda % 16 == 0 && ldw % 16 == 0 && ldc % 8 == 0, LX2V_EINVAL, "gemm_fp8_block128: fp8 row strides must be multiples of 16, ldc of 8");
   LX2V_REQUIRE(lda >= K && ldw >= K && ldc >= N, LX2V_EINVAL, "gemm_fp8_block128: row stride smaller than the row length");
   LX2V_REQUIRE(lda < (1LL << 22) && ldw < (1LL << 22), LX2V_EUNSUP, "gemm_fp8_block128: fp8 row strides must be below 4 MiB (a tile's rows are addressed with 31 bits)");
+  LX2V_REQUIRE(ldc < (1LL << 22) && (epilogue != LX2V_EPI_RESIDUAL || ldr < (1LL << 22)), LX2V_EUNSUP, "gemm_fp8_block128: bf16 row strides must be below 4 Mi elements");
   LX2V_REQUIRE(ld_a_scale >= M && ld_w_scale >= (K + BK - 1) / BK, LX2V_EINVAL, "gemm_fp8_block128: ld_a_scale must be >= M, ld_w_scale >= ceil(K / 128)");
   LX2V_REQUIRE(ld_w_scale < (1LL << 28), LX2V_EUNSUP, "gemm_fp8_block128: ld_w_scale=%lld is too large", (long long)ld_w_scale);
   LX2V_REQUIRE(lx2v_aligned16(A) && lx2v_aligned16(W) && lx2v_aligned16(C) && lx2v_aligned16(bias), LX2V_EINVAL, "gemm_fp8_block128: tensors must be 16-byte aligned");
