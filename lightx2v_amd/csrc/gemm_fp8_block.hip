@@ -557,7 +557,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     const auto b_rs = resource(bias_at, bias_at ? (int64_t)N * 4 : 0), g_rs = resource(gate_at, EPI == LX2V_EPI_RESIDUAL && gate_at ? (int64_t)N * 4 : 0);
     // step u = column block pair u / MT, row block u % MT.  Bias and gate are loaded one pair ahead, residual rows RV steps ahead.
     // (the residual form has registers for one pair's bias and gate only)
-    constexpr int U = 4 * MT, RV = 2, CV = EPI == LX2V_EPI_RESIDUAL ? 1 : 2;
+    constexpr int U = 4 * MT, RV = MT, CV = EPI == LX2V_EPI_RESIDUAL ? 1 : 2;
     const int col0 = n0 + wn * 128 + fq_ * 4;
     f32x4 bv[CV][2], gv[CV][2];
     u32x2 rv[RV][2];
@@ -581,12 +581,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
         for (int h = 0; h < 2; ++h) rv[u % RV][h] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r_rs, at + 32 * h, 0, 0));
       }
     };
+    auto store = [&](auto uc, const u32x4& v) __attribute__((always_inline)) {
+      constexpr int u = decltype(uc)::value;
+      const int row = wm * 16 * MT + (u % MT) * 16 + fr_, n = n0 + wn * 128 + (2 * (u / MT) + (fq_ & 1)) * 16 + (fq_ >> 1) * 8;
+      __builtin_amdgcn_raw_buffer_store_b128(v, c_rs, m0 + row < M && n < N ? (row * (int)ldc + n) * 2 : NOWHERE, 0, 0);
+    };
     fetch_cols(IntC<0>{});
     static_for<0, RV>([&](auto uc) __attribute__((always_inline)) { fetch_rows(uc); });
     static_for<0, U>([&](auto uc) __attribute__((always_inline)) {
       constexpr int u = decltype(uc)::value, i = u % MT, k2 = u / MT, b = k2 % CV;
-      if constexpr (CV == 2 && i == 0 && k2 < 3) fetch_cols(IntC<k2 + 1>{});
-      const int row = wm * 16 * MT + i * 16 + fr_;
+      if constexpr (EPI != LX2V_EPI_RESIDUAL && i == 0 && k2 < 3) fetch_cols(IntC<k2 + 1>{});
       uint32_t d[2][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -610,11 +614,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       // with columns 0-7 of block k, row 1 with 0-7 of block k + 1, row 2 with 8-15 of block k, row 3 with 8-15 of block k + 1
       const auto x = __builtin_amdgcn_permlane16_swap(d[0][0], d[1][0], false, false);
       const auto y = __builtin_amdgcn_permlane16_swap(d[0][1], d[1][1], false, false);
-      const int n = n0 + wn * 128 + (2 * k2 + (fq_ & 1)) * 16 + (fq_ >> 1) * 8;
-      const bool in = m0 + row < M && n < N;
-      __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], y[0], x[1], y[1]}, c_rs, in ? (row * (int)ldc + n) * 2 : NOWHERE, 0, 0);
-      if constexpr (CV == 1 && i == MT - 1 && k2 < 3) fetch_cols(IntC<k2 + 1>{});
-      fetch_rows(IntC<u + RV>{});
+      const u32x4 out = {x[0], y[0], x[1], y[1]};
+      if constexpr (EPI != LX2V_EPI_RESIDUAL) {
+        store(uc, out);
+      } else {
+        // Memory operations retire in order: a residual load behind a store would wait for its write.  So the results stay, in
+        // registers of sums that are done with, until all rows are loaded.
+        acc[i][2 * k2] = __builtin_bit_cast(f32x4, out);
+        asm volatile("" : "+v"(acc[i][2 * k2]));
+        fetch_rows(IntC<u + RV>{});
+        if constexpr (i == MT - 1 && k2 < 3) fetch_cols(IntC<k2 + 1>{});
+        if constexpr (u == U - 1) static_for<0, U>([&](auto vc) __attribute__((always_inline)) { store(vc, __builtin_bit_cast(u32x4, acc[decltype(vc)::value % MT][2 * (decltype(vc)::value / MT)])); });
+      }
       asm volatile("" ::: FRAG_CLOBBERS);  // (the next block's fragments are in there: nothing of the epilogue may stay in them)
       __builtin_amdgcn_sched_barrier(0);
     });
