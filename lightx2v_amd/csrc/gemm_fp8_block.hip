@@ -109,158 +109,27 @@ LX2V_DEVICE void finish4(const Params& p, const f32x4& acc, int64_t m, int n) {
   *reinterpret_cast<u32x2*>(p.C + m * p.ldc + n) = u32x2{pack2(v[0], v[1]), pack2(v[2], v[3])};
 }
 
-// ---- tile kernel ------------------------------------------------------------------------------------
-// Workgroup = 4 waves (2 x 2), wave tile 16 MT x 16 NT, a ring of S operand tiles in LDS.  Slot: A rows | W rows (128
-// bytes a row, 16-byte chunk c at position c ^ ((row >> 1) & 7)) | 1 KiB of scales (256 bytes filled by each wave's one
-// 4-byte DMA: waves 0 .. the A scales of 64 rows each, wave 3 the weight scales of the tile's one or two row blocks).
-// A lane's 32 bytes of K are chunks fq and fq + 4 of its row, not two adjacent ones: any split of the 128 bytes serves as long as
-// both operands use the same one, and a ds_read_b128 serves lanes 0-3, 12-15, 20-27 (and so on) together, which with this
-// split fall on different banks and with adjacent chunks on the same ones two by two.
-template <int MT, int NT, int S>
-struct Tile {
+// ---- stream kernel ------------------------------------------------------------------------------------
+// One wave per SIMD, 4 waves (2 x 2), wave tile 16 MT x 16 NT (within one row block of weight scales), persistent: a workgroup
+// walks its output tiles as one stream of K blocks.  Block j is multiplied while block j + 1 is read from LDS into the other
+// set of fragment registers (so the LDS reads are spread over the whole block) and the blocks behind it are on their way into
+// rings of SA A slots and SW W slots: once every wave has block j in registers, its slots take W(j + SW) with its scales and
+// A(j + SA).
+template <int MT_, int NT_, int SA_, int SW_>
+struct Stream {
+  static constexpr int MT = MT_, NT = NT_, SA = SA_, SW = SW_;
   static constexpr int TM = 32 * MT, TN = 32 * NT;
   static constexpr int A_BYTES = TM * BK, W_BYTES = TN * BK;
-  static constexpr int SLOT = A_BYTES + W_BYTES + 1024;
-  static constexpr int LDS = S * SLOT;
-  static constexpr int PA = TM / 32, PW = TN / 32;  // 1 KiB DMA pieces (8 rows) of a wave
-  static constexpr int PIECES = PA + PW + 1;
-};
-
-template <int MT, int NT, int S, int EPI>
-__global__ __launch_bounds__(256) void gemm_fp8_block_tile_kernel(const Params p) {
-  using T = Tile<MT, NT, S>;
-  __shared__ __attribute__((aligned(16))) char lds[T::LDS];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wid >> 1, wn = wid & 1;
-  const int fr = lane & 15, fq = lane >> 4;
-
-  const int item = xcd_remap(blockIdx.x, gridDim.x);
-  const int part = item % p.split, tile = item / p.split;
-  const int group_sz = GROUP_M * p.tiles_n, first_m = tile / group_sz * GROUP_M;
-  const int gm = min(p.tiles_m - first_m, GROUP_M), in_g = tile % group_sz;
-  const int m0 = (first_m + in_g % gm) * T::TM, n0 = in_g / gm * T::TN;
-  const int kb0 = part * p.per, nk = min(p.per, p.nk - kb0);
-
-  const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t)(size_t)(__attribute__((address_space(3))) char*)lds);
-  constexpr int NOWHERE = (int)0x80000000u;  // an offset past the end of every descriptor
-
-  // ---- staging: piece q of wave w fills rows 8 (q * 4 + w) .. + 7 of an operand tile (lane L: row L >> 3, position L & 7)
-  int a_pv[T::PA], w_pv[T::PW];
-  auto chunk_of = [&](int q) __attribute__((always_inline)) { return (lane & 7) ^ (((8 * (q * 4 + wid) + (lane >> 3)) >> 1) & 7); };
-  auto set_voff = [&](bool last) __attribute__((always_inline)) {  // `last`: chunks past K go nowhere
-    const int left = p.K - (p.nk - 1) * BK;
-#pragma unroll
-    for (int q = 0; q < T::PA; ++q) a_pv[q] = last && chunk_of(q) * 16 >= left ? NOWHERE : (8 * (q * 4 + wid) + (lane >> 3)) * (int)p.lda + chunk_of(q) * 16;
-#pragma unroll
-    for (int q = 0; q < T::PW; ++q) w_pv[q] = last && chunk_of(q) * 16 >= left ? NOWHERE : (8 * (q * 4 + wid) + (lane >> 3)) * (int)p.ldw + chunk_of(q) * 16;
-  };
-  set_voff(false);
-  const u32x4 a_rs = raw_descriptor(p.A + (int64_t)m0 * p.lda, min((int64_t)p.M - m0, (int64_t)T::TM) * p.lda);
-  const u32x4 w_rs = raw_descriptor(p.W + (int64_t)n0 * p.ldw, min((int64_t)p.N - n0, (int64_t)T::TN) * p.ldw);
-  const bool sw_wave = wid == 3, sa_wave = wid < (T::TM + 63) / 64;
-  const int nb = min(((p.N + 127) >> 7) - (n0 >> 7), (T::TN + 127) / 128);  // weight row blocks of the tile
-  const int s_pv = sw_wave ? (lane < nb ? lane * (int)p.lds_w * 4 : NOWHERE) : sa_wave ? (64 * wid + lane) * 4 : NOWHERE;
-
-  auto dma16 = [&](uint32_t dst, const u32x4& rs, int voff, uint32_t soff) __attribute__((always_inline)) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(dst)), "v"(voff), "s"(rs), "s"(soff) : "memory");
-  };
-  auto stage = [&](int j) __attribute__((always_inline)) {  // K block kb0 + j -> slot j % S
-    const uint32_t slot = lds_base + (uint32_t)(j % S) * T::SLOT;
-    const int kb = kb0 + j;
-    if (kb == p.nk - 1 && (p.K & (BK - 1)) != 0) set_voff(true);
-    const uint32_t soff = (uint32_t)kb * BK;
-#pragma unroll
-    for (int q = 0; q < T::PA; ++q) dma16(slot + 1024 * (q * 4 + wid), a_rs, a_pv[q], soff);
-#pragma unroll
-    for (int q = 0; q < T::PW; ++q) dma16(slot + T::A_BYTES + 1024 * (q * 4 + wid), w_rs, w_pv[q], soff);
-    const float* sb = sw_wave ? p.w_scale + (int64_t)(n0 >> 7) * p.lds_w + kb : p.a_scale + (int64_t)kb * p.lds_a + m0;
-    const u32x4 s_rs = raw_descriptor(sb, sw_wave ? ((int64_t)(nb - 1) * p.lds_w + 1) * 4 : sa_wave ? ((int64_t)p.M - m0) * 4 : 0);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(slot + T::A_BYTES + T::W_BYTES + 256 * wid)), "v"(s_pv), "s"(s_rs) : "memory");
-  };
-
-  int rd_a[2], rd_w[2];  // the lane's 32 bytes of K: chunks fq and fq + 4 of its row (see Tile); 16 rows on: + 2048 bytes
-  {
-    const int ar = wm * 16 * MT + fr, wr = wn * 16 * NT + fr;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      rd_a[c] = ar * BK + (((fq + 4 * c) ^ ((ar >> 1) & 7)) << 4);
-      rd_w[c] = T::A_BYTES + wr * BK + (((fq + 4 * c) ^ ((wr >> 1) & 7)) << 4);
-    }
-  }
-  auto frag = [&](const char* base, const int (&rd)[2], int i) __attribute__((always_inline)) -> i32x8 {
-    const i32x4 lo = *reinterpret_cast<const i32x4*>(base + rd[0] + i * 2048), hi = *reinterpret_cast<const i32x4*>(base + rd[1] + i * 2048);
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-  };
-
-  f32x4 acc[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int k = 0; k < NT; ++k) acc[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-#pragma unroll
-  for (int j = 0; j < S - 1; ++j)
-    if (j < nk) stage(j);
-  for (int j = 0; j < nk; ++j) {
-    // this wave's pieces of K block j have landed (younger blocks may be in flight); behind the barrier every wave's have, and
-    // every wave has left block j - 1, whose slot block j + S - 1 is staged into
-    if (j + S - 2 < nk) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * T::PIECES) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (j + S - 1 < nk) stage(j + S - 1);
-    const char* slot = lds + (j % S) * T::SLOT;
-    const float* sc = reinterpret_cast<const float*>(slot + T::A_BYTES + T::W_BYTES);
-    const float sw = sc[192 + ((wn * 16 * NT) >> 7)];
-    i32x8 wf[NT];
-#pragma unroll
-    for (int k = 0; k < NT; ++k) wf[k] = frag(slot, rd_w, k);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const i32x8 af = frag(slot, rd_a, i);
-      const float s = sc[wm * 16 * MT + i * 16 + fr] * sw;
-#pragma unroll
-      for (int k = 0; k < NT; ++k) {
-        const f32x4 d = mfma_block(wf[k], af);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][k][e] = __builtin_fmaf(d[e], s, acc[i][k][e]);
-      }
-    }
-  }
-
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int m = m0 + wm * 16 * MT + i * 16 + fr;
-    if (m >= p.M) continue;
-#pragma unroll
-    for (int k = 0; k < NT; ++k) {
-      const int n = n0 + wn * 16 * NT + k * 16 + fq * 4;
-      if (n >= p.N) continue;  // N % 8 == 0: all four columns or none
-      if constexpr (EPI == EPI_PARTIAL) *reinterpret_cast<f32x4*>(p.partials + ((int64_t)part * p.M + m) * p.N + n) = acc[i][k];
-      else finish4<EPI>(p, acc[i][k], m, n);
-    }
-  }
-}
-
-// ---- stream kernel ------------------------------------------------------------------------------------
-// Long products: one wave per SIMD, 4 waves (2 x 2), wave tile 16 MT x 128 (one row block of weight scales), persistent: a
-// workgroup walks its output tiles as one stream of K blocks.  Block j is multiplied while block j + 1 is read from LDS into
-// the other set of fragment registers (so the LDS reads are spread over the whole block) and the blocks behind it are on
-// their way: once every wave has block j in registers, its slots take W(j + 2) and its scales, issued first, which have one
-// block's time to arrive, and A(j + 3), which has two.  LDS: three A slots, two W slots, two of scales.
-template <int MT>
-struct Stream {
-  static constexpr int TM = 32 * MT, TN = 256;
-  static constexpr int A_BYTES = TM * BK, W_BYTES = TN * BK;
-  static constexpr int W_AT = 3 * A_BYTES, S_AT = W_AT + 2 * W_BYTES;
-  static constexpr int LDS = S_AT + 2 * 1024;
+  static constexpr int W_AT = SA * A_BYTES, S_AT = W_AT + SW * W_BYTES;
+  static constexpr int LDS = S_AT + SW * 1024;
+  static_assert(LDS <= 160 * 1024 && SA >= SW && SW >= 2, "LDS of a CU; the order of the waits");
   static constexpr int PA = TM / 32, PW = TN / 32;  // DMA pieces of 1 KiB a wave
-  static constexpr int PIECES = PW + 1 + PA;        // W(j + 2), its scales, A(j + 3)
-  static constexpr int STEPS = 8 * MT;
-  static_assert(STEPS % 3 == 0, "the ring of three results wraps with the block");
-  static_assert(2 * PIECES <= STEPS, "a piece takes two steps");
-  static constexpr int STORES = 4 * MT;
+  static constexpr int PIECES = PW + 1 + PA;        // W(j + SW), its scales, A(j + SA)
+  static constexpr int AHEAD = (SW - 2) * PIECES + (SA > SW ? PA : 0);  // pieces issued behind the last one of block j + 2, at the end of block j
+  static constexpr int STEPS = MT * NT;
+  static constexpr int RES = STEPS % 3 == 0 ? 3 : 4;  // ring of MFMA results
+  static_assert(STEPS % RES == 0, "the ring of results wraps with the block");
+  static constexpr int READS = 2 * NT + 3 * MT + 1;
 };
 
 // n / d and n % d from floor(2^32 / d): the estimate is the quotient or one less.
@@ -316,16 +185,25 @@ LX2V_DEVICE ParamsAgain params_again() {
   "a224", "a225", "a226", "a227", "a228", "a229", "a230", "a231", "a232", "a233", "a234", "a235", "a236", "a237", "a238", "a239", \
   "a240", "a241", "a242", "a243", "a244", "a245", "a246", "a247", "a248", "a249", "a250", "a251", "a252", "a253", "a254", "a255"
 
-template <int MT, int EPI>
+template <class T, int EPI>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void gemm_fp8_block_stream_kernel(const Params p) {
-  using T = Stream<MT>;
+  constexpr int MT = T::MT, NT = T::NT;
+  constexpr int STORES = EPI == EPI_PARTIAL ? MT * NT : MT * NT / 2;
   __shared__ __attribute__((aligned(16))) char lds[T::LDS];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wid >> 1, wn = wid & 1;
   const int fr = lane & 15, fq = lane >> 4;
-  const int ntiles = p.tiles_m * p.tiles_n, grid = gridDim.x, nk = p.nk;
-  const int my_tiles = (int)blockIdx.x < ntiles ? (ntiles - 1 - (int)blockIdx.x) / grid + 1 : 0;
+  const int ntiles = p.tiles_m * p.tiles_n, grid = gridDim.x;
+  // a workgroup's tiles are first, first + grid, ...; EPI_PARTIAL: one K range (blocks kb0 ..) of one tile
+  int first = blockIdx.x, kb0 = 0, nk = p.nk, part_id = 0;
+  if constexpr (EPI == EPI_PARTIAL) {
+    part_id = first / ntiles;
+    first -= part_id * ntiles;
+    kb0 = part_id * p.per;
+    nk = min(p.per, nk - kb0);
+  }
+  const int my_tiles = first < ntiles ? (ntiles - 1 - first) / grid + 1 : 0;
   const int64_t total = (int64_t)my_tiles * nk;
   if (total == 0) return;
 
@@ -334,11 +212,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   constexpr int NOWHERE = (int)0x80000000u;
   const bool sw_wave = wid == 3, sa_wave = wid < (T::TM + 63) / 64;
 
-  // ---- DMA cursors: W and its scales two blocks ahead of the multiplied one, A three ----
+  // ---- DMA cursors: W and its scales SW blocks ahead of the multiplied one, A SA blocks ----
   // piece q of wave w: rows 32 q + 8 w + (lane >> 3) of the operand tile; the swizzle is the same for all q
   const int chunk = (lane & 7) ^ ((4 * wid + (lane >> 4)) & 7);
-  const int left = p.K - (nk - 1) * BK;  // columns of the last block
-  const int ragged = left < BK ? nk - 1 : -1;
+  const int left = p.K - (p.nk - 1) * BK;  // columns of the last block
+  const int ragged = left < BK && kb0 + nk == p.nk ? nk - 1 : -1;
   int a_pv, w_pv, s_pv = NOWHERE;
   auto offset = [&](int64_t ld, bool last) __attribute__((always_inline)) -> int {  // of piece 0; `last`: chunks past K go nowhere
     return last && chunk * 16 >= left ? NOWHERE : (8 * wid + (lane >> 3)) * (int)ld + chunk * 16;
@@ -357,7 +235,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     const int64_t lda = p->lda;
     const int M = p->M;
     asm volatile("" ::"s"(base), "s"(lda), "s"(M));
-    const int vbid = ca.ord * grid + (int)blockIdx.x;
+    const int vbid = ca.ord * grid + first;
     int m0, n0;
     tile_origin(raster, vbid, T::TM, T::TN, m0, n0);
     const int rows = vbid < ntiles ? min(M - m0, T::TM) : 0;
@@ -366,26 +244,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   auto w_tile = [&]() __attribute__((always_inline)) {
     const ParamsAgain p = params_again();
     const uint64_t base = reinterpret_cast<uint64_t>(p->W), asb = reinterpret_cast<uint64_t>(p->a_scale), wsb = reinterpret_cast<uint64_t>(p->w_scale);
-    const int64_t ldw = p->ldw, lds_w = p->lds_w;
+    const int64_t ldw = p->ldw, lds_w = p->lds_w, lds_a = p->lds_a;
     const int M = p->M, N = p->N;
-    asm volatile("" ::"s"(base), "s"(asb), "s"(wsb), "s"(ldw), "s"(lds_w), "s"(M), "s"(N));
-    const int vbid = cw.ord * grid + (int)blockIdx.x;
+    asm volatile("" ::"s"(base), "s"(asb), "s"(wsb), "s"(ldw), "s"(lds_w), "s"(lds_a), "s"(M), "s"(N));
+    const int vbid = cw.ord * grid + first;
     const bool live = vbid < ntiles;
     int m0, n0;
     tile_origin(raster, vbid, T::TM, T::TN, m0, n0);
     if (!live) m0 = n0 = 0;
     const int rows = live ? min(N - n0, T::TN) : 0;
     w_rs = raw_descriptor(reinterpret_cast<const uint8_t*>(base) + (int64_t)n0 * ldw, (int64_t)rows * ldw);
-    const int nb = min(((N + 127) >> 7) - (n0 >> 7), 2);
-    const float* sb = sw_wave ? reinterpret_cast<const float*>(wsb) + (int64_t)(n0 >> 7) * lds_w : reinterpret_cast<const float*>(asb) + m0;
+    const int nb = min(((N + 127) >> 7) - (n0 >> 7), (T::TN + 127) / 128);  // weight row blocks of the tile
+    const float* sb = sw_wave ? reinterpret_cast<const float*>(wsb) + (int64_t)(n0 >> 7) * lds_w + kb0 : reinterpret_cast<const float*>(asb) + (int64_t)kb0 * lds_a + m0;
     s_rs = raw_descriptor(sb, !live ? 0 : sw_wave ? ((int64_t)(nb - 1) * lds_w + 1) * 4 : sa_wave ? ((int64_t)M - m0) * 4 : 0);
     s_base = ((uint64_t)s_rs[1] << 32) | s_rs[0];
     s_pv = sw_wave ? (lane < nb ? lane * (int)lds_w * 4 : NOWHERE) : (64 * wid + lane) * 4;
   };
   a_tile();
   w_tile();
-  a_pv = offset(p.lda, nk == 1);
-  w_pv = offset(p.ldw, nk == 1);
+  a_pv = offset(p.lda, ragged == 0);
+  w_pv = offset(p.ldw, ragged == 0);
+  ca.soff = cw.soff = (uint32_t)kb0 * BK;
   {
     const int64_t step = sw_wave ? 4 : p.lds_a * 4;
     s_step = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)step >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)step);
@@ -396,12 +275,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(rs), "s"(soff) : "memory");
   };
   auto load4 = [&](const u32x4& rs, int voff) __attribute__((always_inline)) { asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rs) : "memory"); };
-  // piece q of a block's DMA, its target and then the load itself: W(j + 2), its scales, both into slot P, and A(j + 3) into the A slot at a_cur
-  uint32_t a_cur = dma_base, a_nxt = dma_base + T::A_BYTES;
+  // Ring positions: of block j, which the DMA refills, and of block j + 1, which is read.  (Two W slots: W and the scales of block j
+  // lie at the parity P of j, known at compile time.)
+  uint32_t a_cur = dma_base, a_nxt = dma_base + T::A_BYTES, w_cur = dma_base, w_nxt = dma_base + T::W_BYTES, s_cur = dma_sc, s_nxt = dma_sc + 1024;
+  constexpr bool TWO = T::SW == 2;
+  // piece q of a block's DMA, its target and then the load itself: W(j + SW), its scales, A(j + SA)
   auto dma_set = [&](auto Pc, auto qc) __attribute__((always_inline)) {
     constexpr int P = decltype(Pc)::value, q = decltype(qc)::value;
-    if constexpr (q < T::PW) set_m0(dma_base, IntC<T::W_AT + P * T::W_BYTES + 4096 * q>{});
-    else if constexpr (q == T::PW) set_m0(dma_sc, IntC<T::S_AT + P * 1024>{});
+    if constexpr (q < T::PW) set_m0(TWO ? dma_base : w_cur, IntC<T::W_AT + (TWO ? P * T::W_BYTES : 0) + 4096 * q>{});
+    else if constexpr (q == T::PW) set_m0(TWO ? dma_sc : s_cur, IntC<T::S_AT + (TWO ? P * 1024 : 0)>{});
     else set_m0(a_cur, IntC<4096 * (q - T::PW - 1)>{});
   };
   const int a_step = 32 * (int)p.lda, w_step = 32 * (int)p.ldw;
@@ -433,7 +315,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       cw.soff = 0;
       ++cw.ord;
       w_tile();
-      if (ragged >= 0) w_pv = offset(params_again()->ldw, nk == 1);
+      if (ragged >= 0) w_pv = offset(params_again()->ldw, ragged == 0);
+    }
+    if constexpr (!TWO) {
+      w_cur = w_nxt;
+      w_nxt = w_nxt == dma_base + (T::SW - 1) * T::W_BYTES ? dma_base : w_nxt + T::W_BYTES;
+      s_cur = s_nxt;
+      s_nxt = s_nxt == dma_sc + (T::SW - 1) * 1024 ? dma_sc : s_nxt + 1024;
+      asm volatile("" : "+s"(w_cur), "+s"(w_nxt), "+s"(s_cur), "+s"(s_nxt));
     }
     asm volatile("" : "+s"(w_rs), "+s"(s_rs), "+s"(s_base), "+s"(cw.soff), "+s"(cw.kt), "+s"(cw.ord), "+s"(dma_base), "+s"(dma_sc));
   };
@@ -446,31 +335,38 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       ca.soff = 0;
       ++ca.ord;
       a_tile();
-      if (ragged >= 0) a_pv = offset(params_again()->lda, nk == 1);
+      if (ragged >= 0) a_pv = offset(params_again()->lda, ragged == 0);
     }
     a_cur = a_nxt;
-    a_nxt = a_nxt == dma_base + 2 * T::A_BYTES ? dma_base : a_nxt + T::A_BYTES;
+    a_nxt = a_nxt == dma_base + (T::SA - 1) * T::A_BYTES ? dma_base : a_nxt + T::A_BYTES;
     asm volatile("" : "+s"(a_rs), "+s"(ca.soff), "+s"(ca.kt), "+s"(ca.ord), "+s"(a_cur), "+s"(a_nxt));
   };
 
-  // ---- fragments: register set P (0 | 1) = 8 W fragments, then MT A fragments, of 8 accumulator registers each ----
-  int rd_a[2], rd_w[2];  // LDS addresses of the lane's two 16-byte halves at row block 0 of slot 0 (A: less this wave's share of the DMA target)
+  // ---- fragments: register set P (0 | 1) = NT W fragments, then MT A fragments, of 8 accumulator registers each ----
+  int rd_a[2], rd_w[2];  // LDS addresses of the lane's two 16-byte halves at row block 0 of slot 0 (less this wave's share of a DMA target)
   {
-    const int ar = wm * 16 * MT + fr, wr = wn * 128 + fr;
+    const int ar = wm * 16 * MT + fr, wr = wn * 16 * NT + fr;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       rd_a[c] = ar * BK + (((fq + 4 * c) ^ ((ar >> 1) & 7)) << 4) - 1024 * wid;
-      rd_w[c] = (int)lds_base + T::W_AT + wr * BK + (((fq + 4 * c) ^ ((wr >> 1) & 7)) << 4);
+      rd_w[c] = (TWO ? (int)lds_base : -1024 * wid) + T::W_AT + wr * BK + (((fq + 4 * c) ^ ((wr >> 1) & 7)) << 4);
     }
   }
-  const char* rd_s = lds + T::S_AT + (wm * 16 * MT + fr) * 4;
-  const char* rd_sw = lds + T::S_AT + 768 + wn * 4;
-  int at_a[2];  // rd_a in the slot being read
-  constexpr int FRAG0 = 32, SET = 8 * (8 + MT);
-  static_assert(FRAG0 + 2 * SET <= 256, "fragments exceed the accumulator registers");
+  const int rd_s = T::S_AT + (wm * 16 * MT + fr) * 4, rd_sw = T::S_AT + 768 + ((wn * 16 * NT) >> 7) * 4;
+  int at_a[2], at_w[2], at_s = 0;  // where block j + 1 is read (at_s: the offset of its scales' slot)
+  auto set_reads = [&](uint32_t a_at, uint32_t w_at, uint32_t s_at) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      at_a[c] = rd_a[c] + (int)a_at;
+      at_w[c] = TWO ? rd_w[c] : rd_w[c] + (int)w_at;
+    }
+    if constexpr (!TWO) at_s = (int)(s_at - dma_sc);
+  };
+  constexpr int SET = 8 * (NT + MT), FRAG0 = 256 - 2 * SET;
+  static_assert(FRAG0 >= 32, "fragments exceed the accumulator registers");
   float sa[MT], sw, s[MT], s_last;
-  f32x4 acc[MT][8];
-  f32x4 part[3];
+  f32x4 acc[MT][NT];
+  f32x4 part[T::RES];
   // `old`, the result of the MFMA two before: handed through the statement, so that its additions stay behind this one --
   // 64 cycles at least after the instruction that made it, which the compiler, not knowing what it is, would not wait for
   auto mm = [&](f32x4& d, f32x4& old, auto wc, auto ac) __attribute__((always_inline)) {
@@ -480,55 +376,62 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   auto add = [&](auto tc, float sc, auto FIRSTc) __attribute__((always_inline)) {  // FIRST: the output tile's first block sets the sums
     constexpr int t = decltype(tc)::value;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[t / 8][t % 8][e] = decltype(FIRSTc)::value ? part[t % 3][e] * sc : __builtin_fmaf(part[t % 3][e], sc, acc[t / 8][t % 8][e]);
-    asm volatile("" : "+v"(acc[t / 8][t % 8]));  // (pinned here: without a use the sums would sink to the end of the block and keep every result alive)
+    for (int e = 0; e < 4; ++e) acc[t / NT][t % NT][e] = decltype(FIRSTc)::value ? part[t % T::RES][e] * sc : __builtin_fmaf(part[t % T::RES][e], sc, acc[t / NT][t % NT][e]);
+    asm volatile("" : "+v"(acc[t / NT][t % NT]));  // (pinned here: without a use the sums would sink to the end of the block and keep every result alive)
   };
   auto lds_frag = [&](int addr, auto dstc, auto ofsc) __attribute__((always_inline)) {  // 16 bytes a lane into four accumulator registers; waited for at the next barrier
     asm volatile("ds_read_b128 a[%1:%2], %0 offset:%3" ::"v"(addr), "n"(decltype(dstc)::value), "n"(decltype(dstc)::value + 3), "n"(decltype(ofsc)::value) : "memory", FRAG_CLOBBERS);
   };
-  // LDS read r of a block into register set P: 16 halves of W, 2 MT of A, MT + 1 scales
+  // LDS read r of a block into register set P: 2 NT halves of W, 2 MT of A, MT + 1 scales
   auto rd = [&](auto Pc, auto rc) __attribute__((always_inline)) {
     constexpr int P = decltype(Pc)::value, r = decltype(rc)::value;
-    if constexpr (r < 16) lds_frag(rd_w[r & 1], IntC<FRAG0 + P * SET + 4 * r>{}, IntC<P * T::W_BYTES + (r >> 1) * 2048>{});
-    else if constexpr (r < 16 + 2 * MT) lds_frag(at_a[r & 1], IntC<FRAG0 + P * SET + 4 * r>{}, IntC<((r - 16) >> 1) * 2048>{});
-    else if constexpr (r < 16 + 3 * MT) sa[r - 16 - 2 * MT] = *reinterpret_cast<const float*>(rd_s + P * 1024 + (r - 16 - 2 * MT) * 64);
-    else if constexpr (r == 16 + 3 * MT) sw = *reinterpret_cast<const float*>(rd_sw + P * 1024);
+    if constexpr (r < 2 * NT) lds_frag(at_w[r & 1], IntC<FRAG0 + P * SET + 4 * r>{}, IntC<(TWO ? P * T::W_BYTES : 0) + (r >> 1) * 2048>{});
+    else if constexpr (r < 2 * NT + 2 * MT) lds_frag(at_a[r & 1], IntC<FRAG0 + P * SET + 4 * r>{}, IntC<((r - 2 * NT) >> 1) * 2048>{});
+    else if constexpr (r < 2 * NT + 3 * MT) sa[r - 2 * NT - 2 * MT] = *reinterpret_cast<const float*>(lds + (TWO ? P * 1024 : at_s) + rd_s + (r - 2 * NT - 2 * MT) * 64);
+    else if constexpr (r == 2 * NT + 3 * MT) sw = *reinterpret_cast<const float*>(lds + (TWO ? P * 1024 : at_s) + rd_sw);
   };
-  constexpr int READS = 17 + 3 * MT;
 
   // One block: multiply register set P, read the next one's fragments into set 1 - P, stage into the slots of this one.
   auto block = [&](auto Pc, auto FIRSTc, bool relaxed) __attribute__((always_inline)) {
     constexpr int P = decltype(Pc)::value, Q = 1 - P;
     // the next block is complete in LDS once every wave is past this barrier, and every wave has read its fragments of this one
     // (what was issued behind the next block's last pieces may still be on its way: the pieces of the block after it, an epilogue's stores)
-    if (relaxed) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::PA + T::STORES) : "memory");
-    else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::PA) : "memory");
+    if (relaxed) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::AHEAD + STORES) : "memory");
+    else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::AHEAD) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    at_a[0] = rd_a[0] + (int)a_nxt;
-    at_a[1] = rd_a[1] + (int)a_nxt;
+    set_reads(a_nxt, w_nxt, s_nxt);
     s_last = s[MT - 1];
 #pragma unroll
     for (int i = 0; i < MT; ++i) s[i] = sa[i] * sw;
     static_for<0, T::STEPS>([&](auto tc) __attribute__((always_inline)) {
       constexpr int t = decltype(tc)::value;
-      mm(part[t % 3], part[(t + 1) % 3], IntC<FRAG0 + P * SET + 8 * (t % 8)>{}, IntC<FRAG0 + P * SET + 64 + 8 * (t / 8)>{});
-      // Behind the MFMA its shadow of 32 cycles is filled with the four additions (16) and at most three more instructions: a
-      // piece's target with two LDS reads in an even step, its load in the next one; the reads left follow, two a step, early enough
-      // to be complete at the block's end.
-      if constexpr (t < 2 * T::PIECES) {
-        if constexpr (t % 2 == 0) dma_set(IntC<P>{}, IntC<t / 2>{});
-        else dma_go(IntC<t / 2>{});
-      }
-      if constexpr (t % 2 == 0 || t >= 2 * T::PIECES) {
-        constexpr int r = t < 2 * T::PIECES ? t : 2 * t - 2 * T::PIECES;
-        if constexpr (r < READS) rd(IntC<Q>{}, IntC<r>{});
-        if constexpr (r + 1 < READS) rd(IntC<Q>{}, IntC<r + 1>{});
+      mm(part[t % T::RES], part[(t + T::RES - 2) % T::RES], IntC<FRAG0 + P * SET + 8 * (t % NT)>{}, IntC<FRAG0 + P * SET + 8 * NT + 8 * (t / NT)>{});
+      if constexpr (2 * T::PIECES <= T::STEPS) {
+        // Behind the MFMA its shadow of 32 cycles is filled with the four additions (16) and at most three more instructions: a
+        // piece's target with two LDS reads in an even step, its load in the next one; the reads left follow, two a step, early
+        // enough to be complete at the block's end.
+        if constexpr (t < 2 * T::PIECES) {
+          if constexpr (t % 2 == 0) dma_set(IntC<P>{}, IntC<t / 2>{});
+          else dma_go(IntC<t / 2>{});
+        }
+        if constexpr (t % 2 == 0 || t >= 2 * T::PIECES) {
+          constexpr int r = t < 2 * T::PIECES ? t : 2 * t - 2 * T::PIECES;
+          static_for<r, r + 2>([&](auto rc) __attribute__((always_inline)) { rd(IntC<Q>{}, rc); });
+        }
+      } else {  // few MFMAs: pieces spread over the steps, reads over the first three quarters of them
+        static_for<t * T::PIECES / T::STEPS, (t + 1) * T::PIECES / T::STEPS>([&](auto qc) __attribute__((always_inline)) {
+          dma_set(IntC<P>{}, qc);
+          asm volatile("s_nop 0");
+          dma_go(qc);
+        });
+        constexpr int E = T::STEPS * 3 / 4, r0 = t * T::READS / E, r1 = (t + 1) * T::READS / E;
+        static_for<(r0 < T::READS ? r0 : T::READS), (r1 < T::READS ? r1 : T::READS)>([&](auto rc) __attribute__((always_inline)) { rd(IntC<Q>{}, rc); });
       }
       __builtin_amdgcn_sched_barrier(0);
       constexpr int last = T::STEPS - 2 + t;
-      if constexpr (t >= 2) add(IntC<t - 2>{}, s[(t - 2) / 8], FIRSTc);
-      else if constexpr (decltype(FIRSTc)::value) acc[last / 8][last % 8] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (t >= 2) add(IntC<t - 2>{}, s[(t - 2) / NT], FIRSTc);
+      else if constexpr (decltype(FIRSTc)::value) acc[last / NT][last % NT] = f32x4{0.f, 0.f, 0.f, 0.f};
       else add(IntC<last>{}, s_last, FIRSTc);  // the previous block's last two
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -537,7 +440,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   // ---- epilogue: a lane's four columns become eight consecutive ones by swapping lane rows between two column blocks;
   // 16-byte stores through a descriptor of the tile's rows: rows past M and columns past N are dropped ----
   auto epilogue = [&](int m0, int n0) __attribute__((always_inline)) {
-    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" : "+v"(part[0]), "+v"(part[1]), "+v"(part[2]));  // the last MFMAs were issued a few cycles ago
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" : "+v"(part[(T::STEPS - 2) % T::RES]), "+v"(part[(T::STEPS - 1) % T::RES]));  // the last MFMAs were issued a few cycles ago
     add(IntC<T::STEPS - 2>{}, s[MT - 1], IntC<0>{});
     add(IntC<T::STEPS - 1>{}, s[MT - 1], IntC<0>{});
     const ParamsAgain p = params_again();
@@ -547,6 +450,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     asm volatile("" ::"s"(c_at), "s"(bias_at), "s"(gate_at), "s"(resid_at), "s"(ldc), "s"(ldr), "s"(M), "s"(N));
     int fr_ = fr, fq_ = fq;
     asm volatile("" : "+v"(fr_), "+v"(fq_));
+    if constexpr (EPI == EPI_PARTIAL) {
+      const u32x4 d = raw_descriptor(p->partials + ((int64_t)part_id * M + m0) * N, (int64_t)min(M - m0, T::TM) * N * 4);
+      const auto o_rs = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)d[1] << 32) | d[0]), 0, (int)d[2], 0x00020000);
+      static_for<0, MT * NT>([&](auto uc) __attribute__((always_inline)) {
+        constexpr int i = decltype(uc)::value / NT, k = decltype(uc)::value % NT;
+        const int row = wm * 16 * MT + i * 16 + fr_, n = n0 + wn * 16 * NT + k * 16 + fq_ * 4;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[i][k]), o_rs, m0 + row < M && n < N ? (row * N + n) * 4 : NOWHERE, 0, 0);
+      });
+      return;
+    }
     auto resource = [](uint64_t at, int64_t bytes) __attribute__((always_inline)) {  // accesses past the end: loads give 0, stores are dropped
       const u32x4 d = raw_descriptor(reinterpret_cast<const void*>(at), bytes);
       return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)d[1] << 32) | d[0]), 0, (int)d[2], 0x00020000);
@@ -557,8 +470,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     const auto b_rs = resource(bias_at, bias_at ? (int64_t)N * 4 : 0), g_rs = resource(gate_at, EPI == LX2V_EPI_RESIDUAL && gate_at ? (int64_t)N * 4 : 0);
     // step u = column block pair u / MT, row block u % MT.  Bias and gate are loaded one pair ahead, residual rows RV steps ahead.
     // (the residual form has registers for one pair's bias and gate only)
-    constexpr int U = 4 * MT, RV = MT, CV = EPI == LX2V_EPI_RESIDUAL ? 1 : 2;
-    const int col0 = n0 + wn * 128 + fq_ * 4;
+    constexpr int U = MT * NT / 2, RV = MT, CV = EPI == LX2V_EPI_RESIDUAL ? 1 : 2;
+    const int col0 = n0 + wn * 16 * NT + fq_ * 4;
     f32x4 bv[CV][2], gv[CV][2];
     u32x2 rv[RV][2];
     auto fetch_cols = [&](auto kc) __attribute__((always_inline)) {
@@ -583,14 +496,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     };
     auto store = [&](auto uc, const u32x4& v) __attribute__((always_inline)) {
       constexpr int u = decltype(uc)::value;
-      const int row = wm * 16 * MT + (u % MT) * 16 + fr_, n = n0 + wn * 128 + (2 * (u / MT) + (fq_ & 1)) * 16 + (fq_ >> 1) * 8;
+      const int row = wm * 16 * MT + (u % MT) * 16 + fr_, n = n0 + wn * 16 * NT + (2 * (u / MT) + (fq_ & 1)) * 16 + (fq_ >> 1) * 8;
       __builtin_amdgcn_raw_buffer_store_b128(v, c_rs, m0 + row < M && n < N ? (row * (int)ldc + n) * 2 : NOWHERE, 0, 0);
     };
     fetch_cols(IntC<0>{});
     static_for<0, RV>([&](auto uc) __attribute__((always_inline)) { fetch_rows(uc); });
     static_for<0, U>([&](auto uc) __attribute__((always_inline)) {
       constexpr int u = decltype(uc)::value, i = u % MT, k2 = u / MT, b = k2 % CV;
-      if constexpr (EPI != LX2V_EPI_RESIDUAL && i == 0 && k2 < 3) fetch_cols(IntC<k2 + 1>{});
+      if constexpr (EPI != LX2V_EPI_RESIDUAL && i == 0 && k2 < NT / 2 - 1) fetch_cols(IntC<k2 + 1>{});
       uint32_t d[2][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -623,7 +536,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
         acc[i][2 * k2] = __builtin_bit_cast(f32x4, out);
         asm volatile("" : "+v"(acc[i][2 * k2]));
         fetch_rows(IntC<u + RV>{});
-        if constexpr (i == MT - 1 && k2 < 3) fetch_cols(IntC<k2 + 1>{});
+        if constexpr (i == MT - 1 && k2 < NT / 2 - 1) fetch_cols(IntC<k2 + 1>{});
         if constexpr (u == U - 1) static_for<0, U>([&](auto vc) __attribute__((always_inline)) { store(vc, __builtin_bit_cast(u32x4, acc[decltype(vc)::value % MT][2 * (decltype(vc)::value / MT)])); });
       }
       asm volatile("" ::: FRAG_CLOBBERS);  // (the next block's fragments are in there: nothing of the epilogue may stay in them)
@@ -631,28 +544,23 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     });
   };
 
-  // ---- prologue: W(0), W(1) and their scales, A(0), A(1), A(2), then the fragments of block 0 ----
-  auto piece = [&](auto Pc, auto qc) __attribute__((always_inline)) {
-    dma_set(Pc, qc);
-    asm volatile("s_nop 0");
-    dma_go(qc);
-  };
-  static_for<0, 3>([&](auto bc) __attribute__((always_inline)) {
+  // ---- prologue: the first SW W tiles and their scales, the first SA A tiles, then the fragments of block 0 ----
+  static_for<0, T::SA>([&](auto bc) __attribute__((always_inline)) {
     constexpr int b = decltype(bc)::value;
-    if constexpr (b < 2) {
-      static_for<0, T::PW + 1>([&](auto qc) __attribute__((always_inline)) { piece(bc, qc); });
-      w_advance();
-    }
-    static_for<T::PW + 1, T::PIECES>([&](auto qc) __attribute__((always_inline)) { piece(IntC<0>{}, qc); });
+    static_for<(b < T::SW ? 0 : T::PW + 1), T::PIECES>([&](auto qc) __attribute__((always_inline)) {
+      dma_set(IntC<b & 1>{}, qc);
+      asm volatile("s_nop 0");
+      dma_go(qc);
+    });
+    if constexpr (b < T::SW) w_advance();
     a_advance();
   });
-  // (the ring is back at slot 0: block 0's)
+  // (the rings are back at slot 0: block 0's)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  at_a[0] = rd_a[0] + (int)a_cur;
-  at_a[1] = rd_a[1] + (int)a_cur;
-  static_for<0, READS>([&](auto rc) __attribute__((always_inline)) { rd(IntC<0>{}, rc); });
+  set_reads(a_cur, w_cur, s_cur);
+  static_for<0, T::READS>([&](auto rc) __attribute__((always_inline)) { rd(IntC<0>{}, rc); });
 
   int ord = 0, kt = 0;
   bool relaxed = false;
@@ -664,7 +572,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     relaxed = false;
     if (++kt == nk) {
       int m0, n0;
-      tile_origin(raster, ord * grid + (int)blockIdx.x, T::TM, T::TN, m0, n0);
+      tile_origin(raster, ord * grid + first, T::TM, T::TN, m0, n0);
       epilogue(m0, n0);
       relaxed = true;
       kt = 0;
@@ -690,53 +598,87 @@ __global__ __launch_bounds__(256) void gemm_fp8_block_join_kernel(const Params p
   finish4<EPI>(p, v, m, n);
 }
 
-// ---- skinny kernel: M <= 16 MT ------------------------------------------------------------------------
-// Workgroup = 8 waves on 16 columns; wave w takes K blocks w, w + 8, ...; a weight row's 128 bytes of a block are one
-// cache line, read once, by one wave, into the fragment registers.  The waves' sums meet in LDS in a fixed order.
-template <int MT, int EPI>
+// ---- skinny kernel: M <= 16 MT --------------------------------------------------------------------------
+// The weight is read once and the time goes with its bytes, so it goes straight from memory into fragment registers.  Workgroup =
+// 8 waves on 16 NT columns; wave w takes the K blocks w, w + 8, ..., U of them at a time: all their loads are issued before the
+// first product.  A weight row's 128 bytes of a block are one cache line, read by one wave.  The waves' sums meet in LDS and are
+// added in a fixed order.
+template <int MT, int NT, int U, int EPI>
 __global__ __launch_bounds__(512) void gemm_fp8_block_skinny_kernel(const Params p) {
-  __shared__ __attribute__((aligned(16))) f32x4 red[8][MT][64];
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  __shared__ __attribute__((aligned(16))) f32x4 red[8][MT * NT][64];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int fr = lane & 15, fq = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const uint8_t* wrow = p.W + (int64_t)min(n0 + fr, p.N - 1) * p.ldw + fq * 32;
+  const int n0 = blockIdx.x * 16 * NT;  // (16 NT <= 128 columns inside one row block of weight scales)
+  const uint8_t* wrow[NT];
   const uint8_t* arow[MT];
-  int am[MT];
+  const float* asp[MT];
+#pragma unroll
+  for (int k = 0; k < NT; ++k) wrow[k] = p.W + (int64_t)min(n0 + k * 16 + fr, p.N - 1) * p.ldw + fq * 32;
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
-    am[i] = min(i * 16 + fr, p.M - 1);
-    arow[i] = p.A + (int64_t)am[i] * p.lda + fq * 32;
+    const int m = min(i * 16 + fr, p.M - 1);
+    arow[i] = p.A + (int64_t)m * p.lda + fq * 32;
+    asp[i] = p.a_scale + m;
   }
   const float* swp = p.w_scale + (int64_t)(n0 >> 7) * p.lds_w;
-  f32x4 acc[MT];
+  f32x4 acc[MT][NT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto load = [&](const uint8_t* row, int kb) __attribute__((always_inline)) -> i32x8 {
-    const int k = kb * BK + fq * 32;  // K % 16 == 0: 16 bytes are inside or outside together
-    i32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-    if (k < p.K) lo = *reinterpret_cast<const i32x4*>(row + (int64_t)kb * BK);
-    if (k + 16 < p.K) hi = *reinterpret_cast<const i32x4*>(row + (int64_t)kb * BK + 16);
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int k = 0; k < NT; ++k) acc[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+  struct Frag {
+    i32x4 lo, hi;
   };
-  for (int kb = wid; kb < p.nk; kb += 8) {
-    const i32x8 wf = load(wrow, kb);
-    const float sw = swp[kb];
+  const int k_lane = p.K - fq * 32;  // K % 16 == 0: 16 bytes of a row are inside it or outside it together
+  auto load = [&](const uint8_t* row, int kb, bool nt) __attribute__((always_inline)) -> Frag {
+    Frag f = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    const i32x4* at = reinterpret_cast<const i32x4*>(row + (int64_t)kb * BK);
+    if (kb * BK < k_lane) f.lo = nt ? __builtin_nontemporal_load(at) : at[0];
+    if (kb * BK + 16 < k_lane) f.hi = nt ? __builtin_nontemporal_load(at + 1) : at[1];
+    return f;
+  };
+  auto blocks = [&](auto full, int kb) __attribute__((always_inline)) {
+    Frag wf[U][NT], af[U][MT];
+    float sc[U][MT], sw[U];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const f32x4 d = mfma_block(wf, load(arow[i], kb));
-      const float s = p.a_scale[(int64_t)kb * p.lds_a + am[i]] * sw;
+    for (int u = 0; u < U; ++u) {
+      const int b = kb + 8 * u;
+      const bool in = decltype(full)::value || b < p.nk;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][e] = __builtin_fmaf(d[e], s, acc[i][e]);
+      for (int k = 0; k < NT; ++k) wf[u][k] = in ? load(wrow[k], b, true) : Frag{{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        af[u][i] = in ? load(arow[i], b, false) : Frag{{0, 0, 0, 0}, {0, 0, 0, 0}};
+        sc[u][i] = in ? asp[i][(int64_t)b * p.lds_a] : 0.f;
+      }
+      sw[u] = in ? swp[b] : 0.f;
     }
-  }
 #pragma unroll
-  for (int i = 0; i < MT; ++i) red[wid][i][lane] = acc[i];
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const float s = sc[u][i] * sw[u];
+#pragma unroll
+        for (int k = 0; k < NT; ++k) {
+          const f32x4 d = mfma_block(__builtin_shufflevector(wf[u][k].lo, wf[u][k].hi, 0, 1, 2, 3, 4, 5, 6, 7), __builtin_shufflevector(af[u][i].lo, af[u][i].hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][k][e] = __builtin_fmaf(d[e], s, acc[i][k][e]);
+        }
+      }
+  };
+  int kb = wid;
+  for (; kb + 8 * (U - 1) < p.nk; kb += 8 * U) blocks(IntC<1>{}, kb);
+  if (kb < p.nk) blocks(IntC<0>{}, kb);
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int k = 0; k < NT; ++k) red[wid][i * NT + k][lane] = acc[i][k];
   __syncthreads();
-  if (wid < MT) {
+  if (wid < MT * NT) {
     f32x4 v = red[0][wid][lane];
 #pragma unroll
     for (int w = 1; w < 8; ++w) v += red[w][wid][lane];
-    const int m = wid * 16 + fr, n = n0 + fq * 4;
+    const int m = wid / NT * 16 + fr, n = n0 + wid % NT * 16 + fq * 4;
     if (m < p.M && n < p.N) finish4<EPI>(p, v, m, n);
   }
 }
@@ -754,51 +696,73 @@ int device_cus() {
   return cus;
 }
 
-enum Kind { SKINNY, TILE_64x128, TILE_128x128, TILE_192x256 };
+enum Kind { SKINNY_16, SKINNY_32, SKINNY_64, TILE_64x128, TILE_128x128, TILE_128x256, TILE_192x256 };
 struct Plan {
   Kind kind;
   int tm, tn, split, per;
   int64_t bytes;
 };
 
+// The kernel and split whose estimated time is least.  A tile kernel's time is rounds of one tile (or K range) per CU, each a number
+// of K blocks and an overhead (pipeline fill, epilogue, tile switch); measured on this hardware, one workgroup per CU:
+//   tile        us per K block   us per tile
+//   192 x 256        1.15             5          (one wave's 48 MFMAs are 0.64 us at 2.4 GHz; the rest is memory latency and clock)
+//   128 x 256        0.85             4
+//   128 x 128        0.60             3
+//   64 x 128         0.50             2
+// A split along K adds a launch that reads the partial sums back: 5 us and their bytes, written and read, at 4 TB/s.
 Plan make_plan(int64_t M, int64_t N, int64_t K, int cus) {
   const int nk = (int)((K + BK - 1) / BK);
-  if (M <= 16) return Plan{SKINNY, 16, 16, 1, nk, 0};
-  Plan q{TILE_192x256, 192, 256, 1, nk, 0};
-  auto tiles = [&](int tm, int tn) { return ((M + tm - 1) / tm) * ((N + tn - 1) / tn); };
-  if (tiles(192, 256) < cus) q = Plan{TILE_128x128, 128, 128, 1, nk, 0};
-  if (q.kind == TILE_128x128 && (M <= 64 || tiles(128, 128) < cus)) q = Plan{TILE_64x128, 64, 128, 1, nk, 0};
-  const int64_t t = tiles(q.tm, q.tn);
-  if (q.kind == TILE_64x128 && t < 2 * cus) {
-    int split = (int)std::min<int64_t>(2 * cus / t, std::max(1, nk / 4));
-    const int per = (nk + split - 1) / split;
-    split = (nk + per - 1) / per;
-    if (split > 1) {
-      q.split = split;
-      q.per = per;
-      q.bytes = (int64_t)split * M * N * 4;
+  if (M <= 16) return Plan{SKINNY_16, 16, 16, 1, nk, 0};
+  if (M <= 32) return Plan{SKINNY_32, 32, 32, 1, nk, 0};
+  if (M <= 64) return Plan{SKINNY_64, 64, 32, 1, nk, 0};
+  static const struct {
+    Kind kind;
+    int tm, tn;
+    float block, tile;
+  } kinds[] = {{TILE_192x256, 192, 256, 1.15f, 5.f}, {TILE_128x256, 128, 256, 0.85f, 4.f}, {TILE_128x128, 128, 128, 0.60f, 3.f}, {TILE_64x128, 64, 128, 0.50f, 2.f}};
+  Plan best{TILE_192x256, 192, 256, 1, nk, 0};
+  float least = 1e30f;
+  for (const auto& k : kinds) {
+    const int64_t tiles = ((M + k.tm - 1) / k.tm) * ((N + k.tn - 1) / k.tn);
+    for (int want = 1; want <= 16 && (want == 1 || tiles * want <= cus); ++want) {
+      const int per = (nk + want - 1) / want, split = (nk + per - 1) / per;
+      if (split != want) continue;
+      float t = (float)((tiles * split + cus - 1) / cus) * ((float)per * k.block + k.tile);
+      const int64_t bytes = split > 1 ? (int64_t)split * M * N * 4 : 0;
+      if (split > 1) t += 5.f + (float)bytes * 2e-6f / 4.f;
+      if (t < least) {
+        least = t;
+        best = Plan{k.kind, k.tm, k.tn, split, per, bytes};
+      }
     }
   }
-  return q;
+  return best;
 }
 
-template <int MT, int NT, int S, int EPI>
-void launch_tile(const Params& p, int64_t items, hipStream_t st) {
-  hipLaunchKernelGGL((gemm_fp8_block_tile_kernel<MT, NT, S, EPI>), dim3((unsigned)items), dim3(256), 0, st, p);
+template <int MT, int NT, int U, int EPI>
+void launch_skinny(const Params& p, hipStream_t st) {
+  if constexpr (EPI != EPI_PARTIAL) hipLaunchKernelGGL((gemm_fp8_block_skinny_kernel<MT, NT, U, EPI>), dim3((unsigned)p.tiles_n), dim3(512), 0, st, p);
+}
+
+template <class T, int EPI>
+void launch_stream(const Params& p, int64_t items, hipStream_t st) {
+  // (a K range is one work item of its own workgroup; whole tiles share the CUs' persistent workgroups)
+  const int64_t grid = EPI == EPI_PARTIAL ? items : std::min<int64_t>(items, device_cus());
+  hipLaunchKernelGGL((gemm_fp8_block_stream_kernel<T, EPI>), dim3((unsigned)grid), dim3(256), 0, st, p);
 }
 
 template <int EPI>
 void launch(const Params& p, Kind kind, hipStream_t st) {
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.split;
   switch (kind) {
-    case SKINNY:
-      if constexpr (EPI != EPI_PARTIAL) hipLaunchKernelGGL((gemm_fp8_block_skinny_kernel<1, EPI>), dim3((unsigned)p.tiles_n), dim3(512), 0, st, p);
-      return;
-    case TILE_64x128: return launch_tile<2, 4, 3, EPI>(p, items, st);
-    case TILE_128x128: return launch_tile<4, 4, 2, EPI>(p, items, st);
-    default:
-      if constexpr (EPI != EPI_PARTIAL) hipLaunchKernelGGL((gemm_fp8_block_stream_kernel<6, EPI>), dim3((unsigned)std::min<int64_t>(items, device_cus())), dim3(256), 0, st, p);
-      return;
+    case SKINNY_16: return launch_skinny<1, 1, 4, EPI>(p, st);
+    case SKINNY_32: return launch_skinny<2, 2, 2, EPI>(p, st);
+    case SKINNY_64: return launch_skinny<4, 2, 2, EPI>(p, st);
+    case TILE_64x128: return launch_stream<Stream<2, 4, 6, 6>, EPI>(p, items, st);
+    case TILE_128x128: return launch_stream<Stream<4, 4, 4, 4>, EPI>(p, items, st);
+    case TILE_128x256: return launch_stream<Stream<4, 8, 3, 3>, EPI>(p, items, st);
+    default: return launch_stream<Stream<6, 8, 3, 2>, EPI>(p, items, st);
   }
 }
 

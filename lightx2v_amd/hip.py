@@ -9,6 +9,7 @@ with `torch.cuda.stream(...)`, lightx2v/models/networks/wan/infer/offload/transf
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Optional
 
@@ -776,22 +777,34 @@ class QuantGroups(QuantRows):
     128 columns, `scale` [rows, ceil(dim / 128)] (stored group after group), as `quant_fp8_group128` returns them."""
 
 
-def _launch(entry: str, like: torch.Tensor, *args):
+def _launch(entry: str, device: int, *args):
     """Call an entry point on the current stream of the operands' device (which need not be the current device)."""
-    with torch.cuda.device(like.device):
-        _check(getattr(load(), entry)(*args, _stream()), entry)
+    if device == torch.cuda.current_device():
+        st = getattr(load(), entry)(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            st = getattr(load(), entry)(*args, torch._C._cuda_getCurrentRawStream(device))
+    if st != 0:
+        _check(st, entry)
 
 
 def _need_float_rows(name: str, t: torch.Tensor) -> bool:
     """bf16 or fp32 GPU [rows, dim] with a contiguous innermost dimension; True for fp32."""
     if t.dim() != 2:
         raise Lx2vError(f"{name}: expected [rows, dim], got shape {tuple(t.shape)}")
-    if t.dtype == torch.float32:
+    if t.dtype is torch.float32:
         if not t.is_cuda or (t.stride(1) != 1 and t.shape[1] > 1):
             raise Lx2vError(f"{name}: fp32 input must be a GPU matrix with a contiguous inner dimension")
         return True
     _need_bf16_cuda(name, t)
     return False
+
+
+def _dense_vec(name: str, t: Optional[torch.Tensor], n: int, like: torch.Tensor) -> Optional[torch.Tensor]:
+    """`_vec_f32`, without a view where the vector is one already (most calls: the weights were laid out once)."""
+    if t is not None and t.dtype is torch.float32 and t.dim() == 1 and t.shape[0] == n and t.get_device() == like.get_device() and t.stride(0) == 1:
+        return t
+    return _vec_f32(name, t, n, like)
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -800,8 +813,8 @@ def _row_stride(t: torch.Tensor) -> int:
 
 
 def _group_scales(rows: int, dim: int, device) -> torch.Tensor:
-    """Uninitialised fp32 scales [rows, groups] in the layout of QuantGroups."""
-    return torch.empty(((dim + BLOCK - 1) // BLOCK, rows), dtype=torch.float32, device=device).t()
+    """Uninitialised fp32 scales in memory order, [groups, rows]; the transposed view is QuantGroups' layout."""
+    return torch.empty(((dim + BLOCK - 1) // BLOCK, rows), dtype=torch.float32, device=device)
 
 
 def _group_stride(scale: torch.Tensor) -> int:
@@ -815,25 +828,26 @@ def quant_fp8_group128(x: torch.Tensor, kseg: Optional["KSeg"] = None, dim: Opti
     f32 = _need_float_rows("quant_fp8_group128.x", x)
     if f32 and kseg is not None:
         raise Lx2vError("quant_fp8_group128: a segmented source is bf16")
-    rows = x.shape[0]
-    dim = x.shape[1] if kseg is None else int(dim)
-    q = torch.empty((rows, dim), dtype=torch.float8_e4m3fn, device=x.device)
-    scale = _group_scales(rows, dim, x.device)
-    out = (q.data_ptr(), dim, scale.data_ptr(), _group_stride(scale), rows, dim)
+    rows, width = x.shape
+    dim = width if kseg is None else int(dim)
+    device = x.device
+    q = torch.empty((rows, dim), dtype=torch.float8_e4m3fn, device=device)
+    scale = _group_scales(rows, dim, device)
     if f32:
-        _launch("lx2v_quant_fp8_group128_f32", x, x.data_ptr(), _row_stride(x), *out)
+        _launch("lx2v_quant_fp8_group128_f32", device.index, x.data_ptr(), _row_stride(x), q.data_ptr(), dim, scale.data_ptr(), max(rows, 1), rows, dim)
     else:
-        _launch("lx2v_quant_fp8_group128", x, x.data_ptr(), _row_stride(x), None if kseg is None else ctypes.byref(kseg), *out)
-    return q, scale
+        _launch("lx2v_quant_fp8_group128", device.index, x.data_ptr(), _row_stride(x), None if kseg is None else ctypes.byref(kseg), q.data_ptr(), dim, scale.data_ptr(), max(rows, 1), rows, dim)
+    return q, scale.t()
 
 
 def quant_fp8_block128(w: torch.Tensor):
     """bf16 / fp32 weight [N, K] -> (e4m3 [N, K], fp32 scale [ceil(N / 128), ceil(K / 128)]): one scale per 128 x 128 block."""
     f32 = _need_float_rows("quant_fp8_block128.w", w)
     rows, dim = w.shape
-    q = torch.empty((rows, dim), dtype=torch.float8_e4m3fn, device=w.device)
-    scale = torch.empty(((rows + BLOCK - 1) // BLOCK, (dim + BLOCK - 1) // BLOCK), dtype=torch.float32, device=w.device)
-    _launch("lx2v_quant_fp8_block128_f32" if f32 else "lx2v_quant_fp8_block128", w, w.data_ptr(), _row_stride(w), q.data_ptr(), dim, scale.data_ptr(), scale.shape[1], rows, dim)
+    device, groups = w.device, (dim + BLOCK - 1) // BLOCK
+    q = torch.empty((rows, dim), dtype=torch.float8_e4m3fn, device=device)
+    scale = torch.empty(((rows + BLOCK - 1) // BLOCK, groups), dtype=torch.float32, device=device)
+    _launch("lx2v_quant_fp8_block128_f32" if f32 else "lx2v_quant_fp8_block128", device.index, w.data_ptr(), _row_stride(w), q.data_ptr(), dim, scale.data_ptr(), groups, rows, dim)
     return q, scale
 
 
@@ -849,45 +863,53 @@ def gemm_fp8_block(a8: torch.Tensor, a_scale: torch.Tensor, w8: torch.Tensor, w_
     K % 16 == 0, N % 8 == 0.  `a_scale` as `quant_fp8_group128` lays it out is read in place; another layout is copied first.
     `resid` may be `out`.  `workspace`: uint8 GPU tensor for products that are split along K (`gemm_fp8_block_workspace_bytes`;
     calls that share one must be ordered on one stream); absent, it comes from torch's allocator when one is needed."""
-    dev = a8.device
+    f8, f32 = torch.float8_e4m3fn, torch.float32
+    dev = a8.get_device()   # -1: not a GPU tensor
     for n, t in (("a8", a8), ("w8", w8)):
-        if not t.is_cuda or t.device != dev or t.dtype != torch.float8_e4m3fn or t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+        if dev < 0 or t.get_device() != dev or t.dtype is not f8 or t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
             raise Lx2vError(f"gemm_fp8_block: {n} must be a float8_e4m3fn matrix on one GPU with a contiguous inner dimension, got {t.dtype} {tuple(t.shape)} on {t.device}")
     M, K = a8.shape
-    N = w8.shape[0]
-    if w8.shape[1] != K:
-        raise Lx2vError(f"gemm_fp8_block: K mismatch {K} vs {w8.shape[1]}")
+    N, kw = w8.shape
+    if kw != K:
+        raise Lx2vError(f"gemm_fp8_block: K mismatch {K} vs {kw}")
     groups = (K + BLOCK - 1) // BLOCK
     for n, t, shape in (("a_scale", a_scale, (M, groups)), ("w_scale", w_scale, ((N + BLOCK - 1) // BLOCK, groups))):
-        if t.device != dev or t.dtype != torch.float32 or tuple(t.shape) != shape:
-            raise Lx2vError(f"gemm_fp8_block: {n} must be fp32 {shape} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if t.get_device() != dev or t.dtype is not f32 or t.shape != shape:
+            raise Lx2vError(f"gemm_fp8_block: {n} must be fp32 {shape} on {a8.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     if (M > 1 and a_scale.stride(0) != 1) or (groups > 1 and a_scale.stride(1) < M):
         a_scale = a_scale.t().contiguous().t()
     if not w_scale.is_contiguous():
         w_scale = w_scale.contiguous()
-    bias = _vec_f32("gemm_fp8_block.bias", bias, N, a8)
-    gate = _vec_f32("gemm_fp8_block.gate", gate, N, a8)
+    bias = _dense_vec("gemm_fp8_block.bias", bias, N, a8)
+    gate = _dense_vec("gemm_fp8_block.gate", gate, N, a8)
     if out is None:
-        out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+        out = torch.empty((M, N), dtype=torch.bfloat16, device=a8.device)
+        ldc = N
     else:
         _need_out("gemm_fp8_block.out", out, (M, N), a8)
+        ldc = _row_stride(out)
     if resid is not None:
         _need_out("gemm_fp8_block.resid", resid, (M, N), a8)
     elif epilogue == EPI_RESIDUAL:
         raise Lx2vError("gemm_fp8_block: the residual epilogue needs `resid`")
-    with torch.cuda.device(dev):
-        if workspace is None:
-            need = load().lx2v_gemm_fp8_block128_workspace_bytes(M, N, K)
-            if need > 0:
-                workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        elif workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
-            raise Lx2vError("gemm_fp8_block: workspace must be a contiguous uint8 tensor on the operands' device")
-        st = load().lx2v_gemm_fp8_block128(a8.data_ptr(), _row_stride(a8), a_scale.data_ptr(), _group_stride(a_scale), w8.data_ptr(), _row_stride(w8),
-                                           w_scale.data_ptr(), groups, _ptr(bias), out.data_ptr(), _row_stride(out), M, N, K, epilogue,
-                                           _ptr(resid), 0 if resid is None else _row_stride(resid), _ptr(gate),
-                                           _ptr(workspace), 0 if workspace is None else workspace.numel(), _stream())
-    _check(st, "lx2v_gemm_fp8_block128")
+    if workspace is None:
+        need = _block_workspace_bytes(dev, M, N, K)
+        if need > 0:
+            workspace = torch.empty(need, dtype=torch.uint8, device=a8.device)
+    elif workspace.dtype is not torch.uint8 or workspace.get_device() != dev or not workspace.is_contiguous():
+        raise Lx2vError("gemm_fp8_block: workspace must be a contiguous uint8 tensor on the operands' device")
+    _launch("lx2v_gemm_fp8_block128", dev, a8.data_ptr(), _row_stride(a8), a_scale.data_ptr(), _group_stride(a_scale), w8.data_ptr(), _row_stride(w8),
+            w_scale.data_ptr(), groups, None if bias is None else bias.data_ptr(), out.data_ptr(), ldc, M, N, K, epilogue,
+            None if resid is None else resid.data_ptr(), 0 if resid is None else _row_stride(resid), None if gate is None else gate.data_ptr(),
+            None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel())
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _block_workspace_bytes(device: int, M: int, N: int, K: int) -> int:
+    """The library's answer depends on the shape and the device's CU count alone; asked once per shape."""
+    with torch.cuda.device(device):
+        return gemm_fp8_block_workspace_bytes(M, N, K)
 
 
 _NORM_FORMS = {"row": 0, "group": 1, "int8": 2}  # LX2V_QUANT_*
@@ -900,25 +922,26 @@ def add_rmsnorm_(x: torch.Tensor, y: Optional[torch.Tensor], weight=None, eps: f
     (hip.QuantGroups: e4m3, one scale per 128 columns, for `gemm_fp8_block`) or "int8" (hip.QuantRows of int8, for `gemm_int8`)."""
     f32 = _need_float_rows("add_rmsnorm.x", x)
     rows, dim = x.shape
+    device = x.device
     if y is not None:
         _need_bf16_cuda("add_rmsnorm.y", y)
-        if y.shape != x.shape or y.device != x.device:
-            raise Lx2vError(f"add_rmsnorm: y {tuple(y.shape)} on {y.device} does not match x {tuple(x.shape)} on {x.device}")
-    w = _vec_f32("add_rmsnorm.weight", weight, dim, x)
-    args = (x.data_ptr(), _row_stride(x), _ptr(y), 0 if y is None else _row_stride(y), _ptr(w))
+        if y.shape != x.shape or y.get_device() != device.index:
+            raise Lx2vError(f"add_rmsnorm: y {tuple(y.shape)} on {y.device} does not match x {tuple(x.shape)} on {device}")
+    w = _dense_vec("add_rmsnorm.weight", weight, dim, x)
+    args = (x.data_ptr(), _row_stride(x), None if y is None else y.data_ptr(), 0 if y is None else _row_stride(y), None if w is None else w.data_ptr())
     if quant is None:
         if out is None:
-            out = torch.empty((rows, dim), dtype=torch.bfloat16, device=x.device)
+            out = torch.empty((rows, dim), dtype=torch.bfloat16, device=device)
         else:
             _need_out("add_rmsnorm.out", out, (rows, dim), x)
-        _launch("lx2v_add_rmsnorm_f32" if f32 else "lx2v_add_rmsnorm_bf16", x, *args, out.data_ptr(), _row_stride(out), rows, dim, eps)
+        _launch("lx2v_add_rmsnorm_f32" if f32 else "lx2v_add_rmsnorm_bf16", device.index, *args, out.data_ptr(), _row_stride(out), rows, dim, eps)
         return out
     if out is not None:
         raise Lx2vError("add_rmsnorm: `out` and `quant` exclude each other")
     if quant not in _NORM_FORMS:
         raise Lx2vError(f"add_rmsnorm: quant={quant!r}: None, {', '.join(map(repr, _NORM_FORMS))} are built")
-    q = torch.empty((rows, dim), dtype=torch.int8 if quant == "int8" else torch.float8_e4m3fn, device=x.device)
-    scale = _group_scales(rows, dim, x.device) if quant == "group" else torch.empty((rows,), dtype=torch.float32, device=x.device)
-    _launch("lx2v_add_rmsnorm_quant_f32" if f32 else "lx2v_add_rmsnorm_quant_bf16", x, *args, q.data_ptr(), dim, scale.data_ptr(),
-            _group_stride(scale) if quant == "group" else 0, _NORM_FORMS[quant], rows, dim, eps)
-    return (QuantGroups if quant == "group" else QuantRows)(q, scale)
+    q = torch.empty((rows, dim), dtype=torch.int8 if quant == "int8" else torch.float8_e4m3fn, device=device)
+    scale = _group_scales(rows, dim, device) if quant == "group" else torch.empty((rows,), dtype=torch.float32, device=device)
+    _launch("lx2v_add_rmsnorm_quant_f32" if f32 else "lx2v_add_rmsnorm_quant_bf16", device.index, *args, q.data_ptr(), dim, scale.data_ptr(),
+            max(rows, 1) if quant == "group" else 0, _NORM_FORMS[quant], rows, dim, eps)
+    return QuantGroups(q, scale.t()) if quant == "group" else QuantRows(q, scale)
