@@ -601,11 +601,12 @@ __global__ __launch_bounds__(256) void gemm_fp8_block_join_kernel(const Params p
 // ---- skinny kernel: M <= 16 MT --------------------------------------------------------------------------
 // The weight is read once and the time goes with its bytes, so it goes straight from memory into fragment registers.  Workgroup =
 // 8 waves on 16 NT columns; wave w takes the K blocks w, w + 8, ..., U of them at a time: all their loads are issued before the
-// first product.  A weight row's 128 bytes of a block are one cache line, read by one wave.  The waves' sums meet in LDS and are
+// first product.  (U = 2 or 4, 8 or 16 waves and non-temporal weight loads measure alike.)  A weight row's 128 bytes of a block are one cache line, read by one wave.  The waves' sums meet in LDS and are
 // added in a fixed order.
+constexpr int SKINNY_WAVES = 8;
 template <int MT, int NT, int U, int EPI>
-__global__ __launch_bounds__(512) void gemm_fp8_block_skinny_kernel(const Params p) {
-  __shared__ __attribute__((aligned(16))) f32x4 red[8][MT * NT][64];
+__global__ __launch_bounds__(64 * SKINNY_WAVES) void gemm_fp8_block_skinny_kernel(const Params p) {
+  __shared__ __attribute__((aligned(16))) f32x4 red[SKINNY_WAVES][MT * NT][64];
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int fr = lane & 15, fq = lane >> 4;
   const int n0 = blockIdx.x * 16 * NT;  // (16 NT <= 128 columns inside one row block of weight scales)
@@ -630,11 +631,11 @@ __global__ __launch_bounds__(512) void gemm_fp8_block_skinny_kernel(const Params
     i32x4 lo, hi;
   };
   const int k_lane = p.K - fq * 32;  // K % 16 == 0: 16 bytes of a row are inside it or outside it together
-  auto load = [&](const uint8_t* row, int kb, bool nt) __attribute__((always_inline)) -> Frag {
+  auto load = [&](const uint8_t* row, int kb) __attribute__((always_inline)) -> Frag {
     Frag f = {{0, 0, 0, 0}, {0, 0, 0, 0}};
     const i32x4* at = reinterpret_cast<const i32x4*>(row + (int64_t)kb * BK);
-    if (kb * BK < k_lane) f.lo = nt ? __builtin_nontemporal_load(at) : at[0];
-    if (kb * BK + 16 < k_lane) f.hi = nt ? __builtin_nontemporal_load(at + 1) : at[1];
+    if (kb * BK < k_lane) f.lo = at[0];
+    if (kb * BK + 16 < k_lane) f.hi = at[1];
     return f;
   };
   auto blocks = [&](auto full, int kb) __attribute__((always_inline)) {
@@ -642,13 +643,13 @@ __global__ __launch_bounds__(512) void gemm_fp8_block_skinny_kernel(const Params
     float sc[U][MT], sw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int b = kb + 8 * u;
+      const int b = kb + SKINNY_WAVES * u;
       const bool in = decltype(full)::value || b < p.nk;
 #pragma unroll
-      for (int k = 0; k < NT; ++k) wf[u][k] = in ? load(wrow[k], b, true) : Frag{{0, 0, 0, 0}, {0, 0, 0, 0}};
+      for (int k = 0; k < NT; ++k) wf[u][k] = in ? load(wrow[k], b) : Frag{{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        af[u][i] = in ? load(arow[i], b, false) : Frag{{0, 0, 0, 0}, {0, 0, 0, 0}};
+        af[u][i] = in ? load(arow[i], b) : Frag{{0, 0, 0, 0}, {0, 0, 0, 0}};
         sc[u][i] = in ? asp[i][(int64_t)b * p.lds_a] : 0.f;
       }
       sw[u] = in ? swp[b] : 0.f;
@@ -667,7 +668,7 @@ __global__ __launch_bounds__(512) void gemm_fp8_block_skinny_kernel(const Params
       }
   };
   int kb = wid;
-  for (; kb + 8 * (U - 1) < p.nk; kb += 8 * U) blocks(IntC<1>{}, kb);
+  for (; kb + SKINNY_WAVES * (U - 1) < p.nk; kb += SKINNY_WAVES * U) blocks(IntC<1>{}, kb);
   if (kb < p.nk) blocks(IntC<0>{}, kb);
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -677,7 +678,7 @@ __global__ __launch_bounds__(512) void gemm_fp8_block_skinny_kernel(const Params
   if (wid < MT * NT) {
     f32x4 v = red[0][wid][lane];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) v += red[w][wid][lane];
+    for (int w = 1; w < SKINNY_WAVES; ++w) v += red[w][wid][lane];
     const int m = wid / NT * 16 + fr, n = n0 + wid % NT * 16 + fq * 4;
     if (m < p.M && n < p.N) finish4<EPI>(p, v, m, n);
   }
@@ -696,14 +697,15 @@ int device_cus() {
   return cus;
 }
 
-enum Kind { SKINNY_16, SKINNY_32, SKINNY_64, TILE_64x128, TILE_128x128, TILE_128x256, TILE_192x256 };
+enum Kind { SKINNY_16, SKINNY_32, TILE_64x128, TILE_128x128, TILE_128x256, TILE_192x256 };
 struct Plan {
   Kind kind;
   int tm, tn, split, per;
   int64_t bytes;
 };
 
-// The kernel and split whose estimated time is least.  A tile kernel's time is rounds of one tile (or K range) per CU, each a number
+// Up to 32 rows the skinny kernel (13 x 5120 x 4096: 9.4 us, the 64 x 128 tile split four ways 12.6; 32 x 5120 x 5120: 12.4 and 14.5;
+// at 64 rows its reads of A cost more than they save, 17.4 and 15.5).  Above, the kernel and split whose estimated time is least.  A tile kernel's time is rounds of one tile (or K range) per CU, each a number
 // of K blocks and an overhead (pipeline fill, epilogue, tile switch); measured on this hardware, one workgroup per CU:
 //   tile        us per K block   us per tile
 //   192 x 256        1.15             5          (one wave's 48 MFMAs are 0.64 us at 2.4 GHz; the rest is memory latency and clock)
@@ -715,7 +717,6 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int cus) {
   const int nk = (int)((K + BK - 1) / BK);
   if (M <= 16) return Plan{SKINNY_16, 16, 16, 1, nk, 0};
   if (M <= 32) return Plan{SKINNY_32, 32, 32, 1, nk, 0};
-  if (M <= 64) return Plan{SKINNY_64, 64, 32, 1, nk, 0};
   static const struct {
     Kind kind;
     int tm, tn;
@@ -742,7 +743,7 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int cus) {
 
 template <int MT, int NT, int U, int EPI>
 void launch_skinny(const Params& p, hipStream_t st) {
-  if constexpr (EPI != EPI_PARTIAL) hipLaunchKernelGGL((gemm_fp8_block_skinny_kernel<MT, NT, U, EPI>), dim3((unsigned)p.tiles_n), dim3(512), 0, st, p);
+  if constexpr (EPI != EPI_PARTIAL) hipLaunchKernelGGL((gemm_fp8_block_skinny_kernel<MT, NT, U, EPI>), dim3((unsigned)p.tiles_n), dim3(64 * SKINNY_WAVES), 0, st, p);
 }
 
 template <class T, int EPI>
@@ -756,9 +757,8 @@ template <int EPI>
 void launch(const Params& p, Kind kind, hipStream_t st) {
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.split;
   switch (kind) {
-    case SKINNY_16: return launch_skinny<1, 1, 4, EPI>(p, st);
+    case SKINNY_16: return launch_skinny<1, 1, 2, EPI>(p, st);
     case SKINNY_32: return launch_skinny<2, 2, 2, EPI>(p, st);
-    case SKINNY_64: return launch_skinny<4, 2, 2, EPI>(p, st);
     case TILE_64x128: return launch_stream<Stream<2, 4, 6, 6>, EPI>(p, items, st);
     case TILE_128x128: return launch_stream<Stream<4, 4, 4, 4>, EPI>(p, items, st);
     case TILE_128x256: return launch_stream<Stream<4, 8, 3, 3>, EPI>(p, items, st);
