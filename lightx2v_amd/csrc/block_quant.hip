@@ -17,6 +17,29 @@ namespace {
 constexpr float E4M3_MAX = 448.0f;
 constexpr float AMAX_FLOOR = 1e-12f;
 
+// Non-temporal accesses (BIG) for calls whose tensors are together more than twice the 256 MB memory-side cache, so that
+// nothing of them would be found there again: group quantiser at [75600, 13824] 505 us against 617 without, norm of
+// [75600, 5120] to e4m3 groups 463 against 514.  Below, the producer's result is still there and the consumer finds this
+// one's: norm of [32760, 1536] to e4m3 rows 53 us against 66 with them.
+constexpr int64_t STREAMED_BYTES = 512 << 20;
+template <bool BIG, class V>
+LX2V_DEVICE V ld(const V* p) {
+  return BIG ? __builtin_nontemporal_load(p) : *p;
+}
+template <bool BIG, class V>
+LX2V_DEVICE void st(V* p, const V& v) {
+  if (BIG) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+template <bool BIG>
+LX2V_DEVICE void load8_once(const uint16_t* p, float (&f)[8]) {
+  unpack8(ld<BIG>(reinterpret_cast<const u32x4*>(p)), f);
+}
+template <bool BIG>
+LX2V_DEVICE void load8_once(const float* p, float (&f)[8]) {  // (fp32 rows keep ordinary loads: 3 % faster in the norm of [75600, 5120])
+  load8(p, f);
+}
+
 // All-reduce maximum over the 16 lanes of a DPP row = the 128 columns of one group (8 per lane).
 LX2V_DEVICE float max16(float v) {
 #define LX2V_ROR_MAX(n) v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + (n), 0xf, 0xf, true)))
@@ -48,11 +71,12 @@ LX2V_DEVICE u32x2 cvt8_e4m3(const float (&f)[8], float inv) {
 }
 
 // ---- activations: 1 x 128 groups ------------------------------------------------------------------
-// A wave owns 16 rows x 512 columns (four groups): 16 independent 16-byte loads per lane in flight, the maximum of a
-// group by four DPP rotations, and after the 16 rows the 16 lanes of a group hold one row's scale each, so the
-// transposed scales leave as 64-byte runs.  One read and one write of the data: 3 bytes an element.
-constexpr int QR = 16;
-template <class T>
+// A wave owns 8 rows x 512 columns (four groups): 8 independent 16-byte loads per lane in flight, the maximum of a group by four
+// DPP rotations, and after the 8 rows 8 of the 16 lanes of a group hold one row's scale each, so the transposed scales leave as
+// 32-byte runs.  One read and one write of the data: 3 bytes an element, 6.2 TB/s at [75600, 13824] (16 rows a wave: 4.9, half as
+// many waves fit; 4 rows: 5.7).
+constexpr int QR = 8;
+template <class T, bool BIG>
 __global__ __launch_bounds__(256) void quant_fp8_group128_kernel(const T* x, int64_t ldx, const SegSrc src, uint8_t* out, int64_t ldo, float* scale, int64_t lds,
                                                                  int64_t rows, int dim, int col_tiles) {
   const int lane = threadIdx.x & 63;
@@ -68,14 +92,14 @@ __global__ __launch_bounds__(256) void quant_fp8_group128_kernel(const T* x, int
   for (int i = 0; i < QR; ++i) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[i][j] = 0.f;
-    if (live && i < n) load8(seg_chunk(x, ldx, src, r0 + i, col), f[i]);
+    if (live && i < n) load8_once<BIG>(seg_chunk(x, ldx, src, r0 + i, col), f[i]);
   }
 #pragma unroll
   for (int i = 0; i < QR; ++i) {
     if (i < n) {
-      const float sc = scale_e4m3(max16(absmax8(f[i])));
+      const float sc = scale_e4m3(max16(absmax8(f[i])));  // (lanes past the row's end hold zeros and take part in the rotations)
       if (i == (lane & 15)) keep = sc;
-      if (live) *reinterpret_cast<u32x2*>(out + (r0 + i) * ldo + col) = cvt8_e4m3(f[i], __frcp_rn(sc));
+      if (live) st<BIG>(reinterpret_cast<u32x2*>(out + (r0 + i) * ldo + col), cvt8_e4m3(f[i], __frcp_rn(sc)));
     }
   }
   if ((lane & 15) < n) scale[(int64_t)(col >> 7) * lds + r0 + (lane & 15)] = keep;
@@ -111,19 +135,24 @@ __global__ __launch_bounds__(256) void quant_fp8_block128_kernel(const T* x, int
 }
 
 // ---- residual addition + RMSNorm --------------------------------------------------------------------
-// WPR waves share a row (1: long inputs, one row per wave; 4: few rows, one row per workgroup); the row stays in
-// registers between the two passes, so x and y are read once and x and out written once.  The sum, the statistics and
-// the normalised row are fp32: the norm sees the sum before its rounding to the stream's type, and the 8-bit forms round
-// the fp32 row once, without a bf16 rounding in between.
+// WPR waves share a row, which stays in registers between the two passes, so x and y are read once and x and out written
+// once.  The sum, the statistics and the normalised row are fp32: the norm sees the sum before its rounding to the stream's type, and the 8-bit forms round
+// the fp32 row once, without a bf16 rounding in between.  Bound by memory: 7 bytes an element with bf16 in and out of e4m3
+// (8 of bf16 out), 5.8 TB/s at [75600, 5120].  Four waves a row above 1024 columns: a wave then holds at most 32 columns a lane
+// and enough waves fit to cover the loads (e4m3 groups at [75600, 5120] 463 us against 528 with a wave a row, and a single row
+// of 5120 has 20 loads' latency less); one wave a row up to 1024, where a fourth of the row would leave lanes idle
+// ([65536, 1024] 78 us against 105, [32760, 512] 21 against 30).
 enum { FORM_BF16 = -1, FORM_ROW = LX2V_QUANT_FP8_ROW, FORM_GROUP = LX2V_QUANT_FP8_GROUP128, FORM_INT8 = LX2V_QUANT_INT8_ROW };
 
-LX2V_DEVICE void store8(uint16_t* p, const float (&f)[8]) { *reinterpret_cast<u32x4*>(p) = pack8(f); }
+template <bool BIG>
+LX2V_DEVICE void store8(uint16_t* p, const float (&f)[8]) { st<BIG>(reinterpret_cast<u32x4*>(p), pack8(f)); }
+template <bool BIG>
 LX2V_DEVICE void store8(float* p, const float (&f)[8]) {
-  *reinterpret_cast<f32x4*>(p) = f32x4{f[0], f[1], f[2], f[3]};
-  *reinterpret_cast<f32x4*>(p + 4) = f32x4{f[4], f[5], f[6], f[7]};
+  st<BIG>(reinterpret_cast<f32x4*>(p), f32x4{f[0], f[1], f[2], f[3]});
+  st<BIG>(reinterpret_cast<f32x4*>(p + 4), f32x4{f[4], f[5], f[6], f[7]});
 }
 
-template <class T, int FORM, int WPR, int NC>
+template <class T, int FORM, int WPR, int NC, bool BIG>
 __global__ __launch_bounds__(256) void add_rmsnorm_kernel(T* x, int64_t ldx, const uint16_t* y, int64_t ldy, const float* w, void* out, int64_t ldo, float* scale,
                                                           int64_t lds, int64_t rows, int dim, float eps) {
   constexpr int TPR = 64 * WPR;  // threads per row
@@ -141,10 +170,10 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(T* x, int64_t ldx, con
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[c][j] = 0.f;
     if (ch < nchunks) {
-      load8(xr + ch * 8, f[c]);
+      load8_once<BIG>(xr + ch * 8, f[c]);
       if (y != nullptr) {
         float b[8];
-        load8(y + row * ldy + ch * 8, b);
+        load8_once<BIG>(y + row * ldy + ch * 8, b);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[c][j] += b[j];
       }
@@ -166,7 +195,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(T* x, int64_t ldx, con
   for (int c = 0; c < NC; ++c) {
     const int ch = t + TPR * c;
     if (ch < nchunks) {
-      if (y != nullptr) store8(xr + ch * 8, f[c]);
+      if (y != nullptr) store8<BIG>(xr + ch * 8, f[c]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[c][j] *= rstd;
       if (w != nullptr) {
@@ -175,13 +204,13 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(T* x, int64_t ldx, con
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[c][j] *= g[j];
       }
-      if constexpr (FORM == FORM_BF16) store8(static_cast<uint16_t*>(out) + row * ldo + ch * 8, f[c]);
+      if constexpr (FORM == FORM_BF16) store8<BIG>(static_cast<uint16_t*>(out) + row * ldo + ch * 8, f[c]);
       if constexpr (FORM == FORM_ROW || FORM == FORM_INT8) amax = fmaxf(amax, absmax8(f[c]));
     }
     if constexpr (FORM == FORM_GROUP) {  // (outside the branch: lanes past the row's end hold zeros and take part in the rotations)
       const float sc = scale_e4m3(max16(absmax8(f[c])));
       if (ch < nchunks) {
-        *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(out) + row * ldo + ch * 8) = cvt8_e4m3(f[c], __frcp_rn(sc));
+        st<BIG>(reinterpret_cast<u32x2*>(static_cast<uint8_t*>(out) + row * ldo + ch * 8), cvt8_e4m3(f[c], __frcp_rn(sc)));
         if ((t & 15) == 0) scale[(int64_t)(ch >> 4) * lds + row] = sc;
       }
     }
@@ -210,35 +239,25 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(T* x, int64_t ldx, con
           q[j >> 2] |= ((uint32_t)(int)v & 0xffu) << (8 * (j & 3));
         }
       }
-      *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(out) + row * ldo + ch * 8) = q;
+      st<BIG>(reinterpret_cast<u32x2*>(static_cast<uint8_t*>(out) + row * ldo + ch * 8), q);
     }
   }
 }
 
 template <class T, int FORM>
 void add_rmsnorm_launch(T* x, int64_t ldx, const uint16_t* y, int64_t ldy, const float* w, void* out, int64_t ldo, float* scale, int64_t lds, int64_t rows, int dim, float eps,
-                        hipStream_t st) {
+                        hipStream_t stream) {
   const int nchunks = dim >> 3;
-#define LX2V_ARN(WPR, NC)                                                                                                                              \
-  hipLaunchKernelGGL((add_rmsnorm_kernel<T, FORM, WPR, NC>), dim3((unsigned)((rows + 4 / WPR - 1) / (4 / WPR))), dim3(256), 0, st, x, ldx, y, ldy, w, out, ldo, scale, lds, \
-                     rows, dim, eps)
-  if (rows < 2048) {  // one row per wave would leave most of the 1024 SIMDs without work
-    if (nchunks <= 256) LX2V_ARN(4, 1);
-    else if (nchunks <= 512) LX2V_ARN(4, 2);
-    else if (nchunks <= 768) LX2V_ARN(4, 3);
-    else LX2V_ARN(4, 4);
-    return;
-  }
-  const int need = (nchunks + 63) / 64;
-  if (need <= 1) LX2V_ARN(1, 1);
-  else if (need <= 2) LX2V_ARN(1, 2);
-  else if (need <= 3) LX2V_ARN(1, 3);
-  else if (need <= 4) LX2V_ARN(1, 4);
-  else if (need <= 6) LX2V_ARN(1, 6);
-  else if (need <= 8) LX2V_ARN(1, 8);
-  else if (need <= 10) LX2V_ARN(1, 10);
-  else if (need <= 12) LX2V_ARN(1, 12);
-  else LX2V_ARN(1, 16);
+  const bool big = rows * dim * (int64_t)(sizeof(T) + (y ? 2 : 0) + (FORM == FORM_BF16 ? 2 : 1)) > STREAMED_BYTES;
+#define LX2V_ARN(WPR, NC)                                                                                                                                                      \
+  hipLaunchKernelGGL((big ? add_rmsnorm_kernel<T, FORM, WPR, NC, true> : add_rmsnorm_kernel<T, FORM, WPR, NC, false>), dim3((unsigned)((rows + 4 / WPR - 1) / (4 / WPR))), dim3(256), 0, \
+                     stream, x, ldx, y, ldy, w, out, ldo, scale, lds, rows, dim, eps)
+  if (nchunks <= 64) LX2V_ARN(1, 1);
+  else if (nchunks <= 128) LX2V_ARN(1, 2);
+  else if (nchunks <= 256) LX2V_ARN(4, 1);
+  else if (nchunks <= 512) LX2V_ARN(4, 2);
+  else if (nchunks <= 768) LX2V_ARN(4, 3);
+  else LX2V_ARN(4, 4);
 #undef LX2V_ARN
 }
 
@@ -257,12 +276,12 @@ int add_rmsnorm(const char* what, T* x, int64_t ldx, const uint16_t* y, int64_t 
   LX2V_REQUIRE(form != FORM_GROUP || lds >= rows, LX2V_EINVAL, "%s: the stride between groups of scales must be >= rows", what);
   LX2V_REQUIRE(rows == 0 || static_cast<const void*>(x) != out, LX2V_EINVAL, "%s: out may not be x", what);
   if (rows == 0) return LX2V_OK;
-  hipStream_t st = (hipStream_t)stream;
+  hipStream_t hs = (hipStream_t)stream;
   switch (form) {
-    case FORM_BF16: add_rmsnorm_launch<T, FORM_BF16>(x, ldx, y, ldy, w, out, ldo, scale, lds, rows, dim, eps, st); break;
-    case FORM_ROW: add_rmsnorm_launch<T, FORM_ROW>(x, ldx, y, ldy, w, out, ldo, scale, lds, rows, dim, eps, st); break;
-    case FORM_GROUP: add_rmsnorm_launch<T, FORM_GROUP>(x, ldx, y, ldy, w, out, ldo, scale, lds, rows, dim, eps, st); break;
-    default: add_rmsnorm_launch<T, FORM_INT8>(x, ldx, y, ldy, w, out, ldo, scale, lds, rows, dim, eps, st); break;
+    case FORM_BF16: add_rmsnorm_launch<T, FORM_BF16>(x, ldx, y, ldy, w, out, ldo, scale, lds, rows, dim, eps, hs); break;
+    case FORM_ROW: add_rmsnorm_launch<T, FORM_ROW>(x, ldx, y, ldy, w, out, ldo, scale, lds, rows, dim, eps, hs); break;
+    case FORM_GROUP: add_rmsnorm_launch<T, FORM_GROUP>(x, ldx, y, ldy, w, out, ldo, scale, lds, rows, dim, eps, hs); break;
+    default: add_rmsnorm_launch<T, FORM_INT8>(x, ldx, y, ldy, w, out, ldo, scale, lds, rows, dim, eps, hs); break;
   }
   LX2V_CHECK_LAUNCH(what);
   return LX2V_OK;
@@ -281,7 +300,9 @@ int quant_group128(const T* x, int64_t ldx, const lx2v_kseg* kseg, uint8_t* out,
   const int col_tiles = (dim + 511) / 512;
   const int64_t blocks = ((rows + QR - 1) / QR * col_tiles + 3) / 4;
   LX2V_REQUIRE(blocks < (1LL << 31), LX2V_EUNSUP, "quant_fp8_group128: too many rows");
-  hipLaunchKernelGGL(quant_fp8_group128_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, x, ldx, g, out, ldo, scale, lds, rows, dim, col_tiles);
+  const bool big = rows * dim * (int64_t)(sizeof(T) + 1) > STREAMED_BYTES;
+  auto kernel = big ? quant_fp8_group128_kernel<T, true> : quant_fp8_group128_kernel<T, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, x, ldx, g, out, ldo, scale, lds, rows, dim, col_tiles);
   LX2V_CHECK_LAUNCH("quant_fp8_group128");
   return LX2V_OK;
 }
