@@ -411,7 +411,7 @@ int lx2v_gemm_int8_ws(const int8_t* A, int64_t lda, const float* a_scale, const 
                       const float* gate, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ==== Block-scaled e4m3 Linear: one scale per 128 columns of K ================================
- * The operand form of the reference's "fp8-b128-deepgemm" mm-type (weight in 128 x 128 blocks, activation in groups of
+ * The operand form of the reference's per-block-128 fp8 mm-type (weight in 128 x 128 blocks, activation in groups of
  * 128 channels per token; lightx2v/common/ops/mm/mm_weight.py): parity unpinned, its kernels live in an absent wheel. */
 
 /* ---- activation operand: scale[r, g] = max(max|x[r, 128 g .. 128 g + 127]|, 1e-12) / 448 ; out = e4m3(x * (1 / scale)) ----

@@ -826,8 +826,8 @@ def quant_fp8_group128(x: torch.Tensor, kseg: Optional["KSeg"] = None, dim: Opti
     x ~= q * scale.  The scales lie group after group in memory (the tensor is a transposed view).  `kseg` + `dim` as in
     `quant_fp8_rowwise` (bf16 only)."""
     f32 = _need_float_rows("quant_fp8_group128.x", x)
-    if f32 and kseg is not None:
-        raise Lx2vError("quant_fp8_group128: a segmented source is bf16")
+    if kseg is not None and (f32 or dim is None):
+        raise Lx2vError("quant_fp8_group128: a segmented source is bf16 and needs `dim`")
     rows, width = x.shape
     dim = width if kseg is None else int(dim)
     device = x.device

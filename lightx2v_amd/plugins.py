@@ -7,6 +7,7 @@ reference class it stands in for, so a `WanTransformerInfer`-style caller that o
   ATTN_WEIGHT_REGISTER["hip_flash_attn"]  <-> FlashAttn2Weight / TorchSDPAWeight
         (lightx2v/common/ops/attn/flash_attn.py:29-61, torch_sdpa.py:9-39)
   ATTN_WEIGHT_REGISTER["hip_ulysses"]     <-> UlyssesAttnWeight (ulysses_attn.py:11-137)  [in ulysses.py]
+  MM_WEIGHT_REGISTER["hip-fp8-block128"]  <-> the reference's per-block-128 fp8 scheme (lightx2v/common/ops/mm/mm_weight.py)
   MM_WEIGHT_REGISTER["hip-bf16"]          <-> MMWeight "Default" (lightx2v/common/ops/mm/mm_weight.py:119-201)
   LN_WEIGHT_REGISTER["hip"]               <-> LNWeight "Default" (lightx2v/common/ops/norm/layer_norm_weight.py:135-169)
   RMS_WEIGHT_REGISTER["hip"]              <-> RMSWeightSgl "sgl-kernel" (lightx2v/common/ops/norm/rms_norm_weight.py:112-146)
@@ -206,6 +207,7 @@ class HipMMWeight:
 
     supports_kseg = True  # apply_residual_ can read a K-segmented A operand
     accepts_quantized = False  # input_tensor may be hip.QuantRows (e4m3 rows + per-row scales)
+    norm_form = None  # the 8-bit form `hip.add_rmsnorm_` can hand to this plugin ("row", "group", "int8"), None: bf16 rows
 
     def adopt(self, weight_nk: torch.Tensor, bias: Optional[torch.Tensor]):
         """Use existing storage (e.g. a slice of a fused q|k|v weight) instead of copying."""
@@ -350,6 +352,7 @@ class HipFp8MMWeight(HipMMWeight):
 
     supports_kseg = True  # the row-wise activation quantiser reads the segments and writes the plain e4m3 matrix
     accepts_quantized = True  # a producer that holds whole rows (LayerNorm) may hand over hip.QuantRows
+    norm_form = "row"
 
     def adopt(self, weight_nk, bias, weight_scale=None):
         if weight_scale is None:
@@ -403,6 +406,7 @@ class HipInt8MMWeight(HipFp8MMWeight):
     (:322-330), quantises a bf16 / fp32 weight at load time with the reference's per-channel formula."""
 
     accepts_quantized = False  # the LayerNorm kernel's fused output is e4m3
+    norm_form = "int8"
 
     def load(self, weight_dict):
         w = weight_dict[self.weight_name]
@@ -423,9 +427,77 @@ class HipInt8MMWeight(HipFp8MMWeight):
         raise NotImplementedError("hip-int8: block-streamed (offload) loading is not built")
 
     def _run(self, x, epilogue, resid=None, gate=None, out=None, kseg=None):
-        xq, xs = hip.quant_int8_rowwise(x, kseg=kseg, dim=self.weight_nk.shape[1])
+        if isinstance(x, hip.QuantRows):
+            xq, xs = x.q, x.scale
+        else:
+            xq, xs = hip.quant_int8_rowwise(x, kseg=kseg, dim=self.weight_nk.shape[1])
         return hip.gemm_int8(xq, xs, self.weight_nk, self.weight_scale, self.bias, epilogue=epilogue, resid=resid, gate=gate,
                              out=resid if epilogue == hip.EPI_RESIDUAL else out, workspace=hip.gemm_w8a8_workspace_for(xq, *self.weight_nk.shape))
+
+
+@MM_WEIGHT_REGISTER("hip-fp8-block128")
+class HipFp8Block128MMWeight(HipFp8MMWeight):
+    """Block-scaled e4m3: one fp32 scale per 128 x 128 block of the weight, one per row and 128 columns of the activation
+    (quantised on the way in), fp32 sums, bf16 output -- the operand form of the reference's per-block-128 fp8 scheme
+    (lightx2v/common/ops/mm/mm_weight.py).  Loads a pre-quantised checkpoint (`<name>.weight` in float8_e4m3fn and its
+    scales [ceil(N / 128), ceil(K / 128)] as `<name>.weight_scale` or `<name>.weight_scale_inv`) or quantises a bf16 / fp32
+    weight at load time."""
+
+    accepts_quantized = False  # scales per row do not fit: the activation comes as bf16 rows or as hip.QuantGroups
+    norm_form = "group"
+
+    def load(self, weight_dict):
+        w = weight_dict[self.weight_name]
+        b = weight_dict[self.bias_name] if self.bias_name is not None else None
+        self.bias = _device_ready(b, torch.float32)
+        if w.dtype == torch.float8_e4m3fn:
+            name = self.weight_scale_name if self.weight_scale_name in weight_dict else self.weight_scale_name + "_inv"
+            scale = weight_dict[name].to(torch.float32).contiguous()
+            blocks = tuple((n + hip.BLOCK - 1) // hip.BLOCK for n in w.shape)
+            if tuple(scale.shape) != blocks:
+                raise ValueError(f"hip-fp8-block128: {name} of shape {tuple(scale.shape)}, a weight of {tuple(w.shape)} has one scale per 128 x 128 block: {blocks}")
+            self.weight_nk, self.weight_scale = w.contiguous(), scale
+        else:
+            if not w.is_cuda:
+                if not torch.cuda.is_available():
+                    raise RuntimeError("hip-fp8-block128: quantising a weight at load time runs on the GPU; no GPU is visible (no CPU fallback exists)")
+                w = w.cuda()
+            self.weight_nk, self.weight_scale = hip.quant_fp8_block128((w if w.dtype == COMPUTE_DTYPE else w.to(torch.float32)).contiguous())
+
+    def load_state_dict(self, destination, block_index, adapter_block_index=None):
+        raise NotImplementedError("hip-fp8-block128: block-streamed (offload) loading is not built")
+
+    def adopt(self, weight_nk, bias, weight_scale=None):
+        if weight_scale is None:
+            raise ValueError("hip-fp8-block128: adopting storage needs the block scales with it")
+        self.weight_nk, self.bias, self.weight_scale = weight_nk, bias, weight_scale
+
+    @classmethod
+    def fused(cls, mods):
+        """The members' blocks must stay whole: every member but the last has a multiple of 128 output rows."""
+        if any(m.weight_nk.shape[0] % hip.BLOCK for m in mods[:-1]):
+            raise ValueError(f"hip-fp8-block128: weights of {[m.weight_nk.shape[0] for m in mods]} output rows cannot be fused, a block of 128 rows would span two of them")
+        out = cls(None, None)
+        w = torch.cat([m.weight_nk for m in mods], dim=0).contiguous()
+        b = _cat_bias(mods)
+        sc = torch.cat([m.weight_scale for m in mods], dim=0).contiguous()
+        out.adopt(w, b, sc)
+        o = 0
+        for m in mods:
+            n, blocks = m.weight_nk.shape[0], m.weight_scale.shape[0]
+            m.adopt(w[o:o + n], None if (b is None or m.bias is None) else b[o:o + n], sc[o // hip.BLOCK:o // hip.BLOCK + blocks])
+            o += n
+        return out
+
+    def _run(self, x, epilogue, resid=None, gate=None, out=None, kseg=None):
+        if isinstance(x, hip.QuantGroups):
+            xq, xs = x.q, x.scale
+        elif isinstance(x, hip.QuantRows):
+            raise hip.Lx2vError("hip-fp8-block128: an activation with one scale per row (hip.QuantRows) does not fit, one per row and 128 columns (hip.QuantGroups) does")
+        else:
+            xq, xs = hip.quant_fp8_group128(x, kseg=kseg, dim=self.weight_nk.shape[1])
+        return hip.gemm_fp8_block(xq, xs, self.weight_nk, self.weight_scale, self.bias, epilogue=epilogue, resid=resid, gate=gate,
+                                  out=resid if epilogue == hip.EPI_RESIDUAL else out)
 
 
 # ----------------------------------------------------------------------------------- norms
@@ -552,6 +624,12 @@ class HipRMSWeight(_NormBase):
     def apply_rope_(self, x2d, rope_cos_sin, head_dim):
         """In place: RMSNorm then per-head interleaved RoPE (one pass over HBM)."""
         return hip.rmsnorm_rope(x2d, self.weight, rope_cos_sin, head_dim=head_dim, eps=self.eps, out=x2d)
+
+    def apply_residual_(self, x2d, y, quant_for=None):
+        """x2d += y in place (y None: x2d as it is), then RMSNorm of the sum.  `quant_for`: the matmul plugin(s) that alone
+        consume the result; when they all take one 8-bit form (`norm_form`), the norm writes that form."""
+        forms = {getattr(c, "norm_form", None) for c in (quant_for if isinstance(quant_for, (list, tuple)) else [quant_for])}
+        return hip.add_rmsnorm_(x2d, y, self.weight, eps=self.eps, quant=forms.pop() if len(forms) == 1 else None)
 
     def apply_(self, x2d):
         return hip.rmsnorm_rope(x2d, self.weight, None, eps=self.eps, out=x2d)

@@ -1,6 +1,6 @@
 """Plain 64-bit / IEEE restatement of the block-scaled e4m3 Linear, its quantisers and the residual RMSNorm, for the tests.
 
-The operand form is the one of the reference's "fp8-b128-deepgemm" scheme (lightx2v/common/ops/mm/mm_weight.py): one fp32
+The operand form is the one of the reference's per-block-128 fp8 scheme (lightx2v/common/ops/mm/mm_weight.py): one fp32
 scale per row and 128 columns of the activation, one per 128 x 128 block of the weight.  Its kernels live in a wheel that is
 absent here: parity unpinned."""
 import math
@@ -18,7 +18,8 @@ def blocks(x, block_rows):
 
 
 def quantise(x, block_rows):
-    """fp32 / bf16 rows -> (e4m3, scale): fp32 arithmetic with one rounding per operation, NaN skipped by the maximum."""
+    """fp32 / bf16 rows -> (e4m3, scale): fp32 arithmetic with one rounding per operation (on the CPU: torch divides a GPU tensor by a
+    number as a product with its reciprocal), NaN skipped by the maximum."""
     rows, cols = x.shape
     b = blocks(x.float(), block_rows)
     amax = torch.where(b.isnan(), torch.zeros_like(b), b.abs()).amax(dim=(1, 3))

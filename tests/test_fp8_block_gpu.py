@@ -3,8 +3,11 @@ formulas of oracle/fp8_block_ref.py.  Tolerances are error bounds of the arithme
 import pytest
 import torch
 
+import lightx2v_amd as L
 from lightx2v_amd import hip
 from oracle import fp8_block_ref as R
+from oracle import wan_block_ref as BR
+from tests.util import case_inputs, cos, load_golden
 
 pytestmark = pytest.mark.gpu
 EPI = {"none": hip.EPI_NONE, "gelu": hip.EPI_GELU_TANH, "residual": hip.EPI_RESIDUAL}
@@ -30,7 +33,10 @@ def _within(got, ref, tol):
 # one row, the skinny kernel's last size and the next, part tiles and full ones of every tile kernel, the split along K;
 # one block of K, less than one, a short last one; N below a block, across its edge, a short last one
 SHAPES = [(1, 8, 16), (1, 64, 128), (1, 5120, 5120), (2, 136, 112), (13, 520, 1456), (16, 256, 4096), (17, 264, 144), (33, 2056, 272), (64, 512, 2048), (65, 128, 1024),
-          (200, 384, 640), (257, 5120, 1280), (512, 1536, 8960), (1000, 2056, 1456), (1111, 4096, 384), (4100, 3080, 208), (9000, 1544, 528), (193, 13824, 5120)]
+          (200, 384, 640), (257, 5120, 1280), (512, 1536, 8960), (1000, 2056, 1456), (1111, 4096, 384), (4100, 3080, 208), (9000, 1544, 528), (193, 13824, 5120),
+          # each tile kernel with one block of K and with two, one tile and several for a workgroup; split along K with a ragged last part
+          (70, 136, 16), (900, 1288, 96), (12001, 136, 16), (577, 4104, 144), (20000, 520, 16), (20000, 520, 144), (12001, 1288, 16), (12001, 1288, 144), (20000, 776, 1040),
+          (40, 512, 2048), (70, 136, 4112), (70, 8200, 4112), (484, 4096, 8976), (151, 8960, 13840)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -314,3 +320,142 @@ def test_two_streams_at_once(cuda):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+def test_past_32_bit_offsets(cuda):
+    """Operands of more than 2^31 (and results of more than 2^32) bytes: the last rows are as right as the first."""
+    rows, dim, n = 320000, 8192, 136
+    g = torch.Generator(device=cuda).manual_seed(41)
+    x = torch.empty((rows, dim), dtype=torch.bfloat16, device=cuda).normal_(generator=g)
+    y = torch.empty_like(x).normal_(generator=g)
+    w = 1 + 0.1 * _rand(g, dim)
+    wq, w_s = hip.quant_fp8_block128(_rand(g, n, dim, std=0.05))
+    pick = torch.tensor([0, 1, 131071, 131072, 262143, 262144, rows - 2, rows - 1], device=cuda)
+    q, s = hip.quant_fp8_group128(x)
+    ref_q, ref_s = (t.to(cuda) for t in R.quantise(x[pick].cpu(), 1))   # on the CPU: torch's GPU quotient of a tensor and a number is not the rounded one
+    assert torch.equal(q[pick].view(torch.uint8), ref_q.view(torch.uint8)) and torch.equal(s[pick], ref_s)
+    ref, tol = R.linear(ref_q, ref_s, wq, w_s)
+    _within(hip.gemm_fp8_block(q, s, wq, w_s)[pick], ref, tol)
+    wide = q[:260000].view(-1, 2 * dim)[:, :dim]      # rows 16 KiB apart
+    ref, tol = R.linear(wide[-3:].contiguous(), s[:260000:2][-3:], wq, w_s)
+    _within(hip.gemm_fp8_block(wide, s[:260000:2], wq, w_s)[-3:], ref, tol)
+    del q, s, wide
+    x0, y0 = x[pick], y[pick]
+    h = hip.add_rmsnorm_(x, y, w, quant="group")
+    small = hip.add_rmsnorm_(x0, y0, w, quant="group")
+    assert torch.equal(x[pick], x0) and torch.equal(h.q[pick].view(torch.uint8), small.q.view(torch.uint8)) and torch.equal(h.scale[pick], small.scale)
+
+
+# ---- the plugin and the blocks that run on it ----
+def _plugin(name, w, b=None, **extra):
+    mm = L.MM_WEIGHT_REGISTER[name]("w.weight", None if b is None else "w.bias")
+    mm.load({"w.weight": w, **({} if b is None else {"w.bias": b}), **extra})
+    return mm
+
+
+def test_plugin_loads_quantises_and_applies(cuda):
+    M, N, K = 77, 328, 400
+    g = torch.Generator(device=cuda).manual_seed(51)
+    x, w, b = _rand(g, M, K).to(torch.bfloat16), _rand(g, N, K, std=0.05), _rand(g, N, std=0.3)
+    resid, gate = _rand(g, M, N).to(torch.bfloat16), _rand(g, N)
+    mm = _plugin("hip-fp8-block128", w, b)
+    wq, w_s = (t.to(cuda) for t in R.quantise(w.cpu(), 128))
+    assert torch.equal(mm.weight_nk.view(torch.uint8), wq.view(torch.uint8)) and torch.equal(mm.weight_scale, w_s)
+    aq, a_s = (t.to(cuda) for t in R.quantise(x.cpu(), 1))
+    for epi, run in (("none", lambda: mm.apply(x)), ("gelu", lambda: mm.apply_gelu(x)), ("residual", lambda: mm.apply_residual_(x, resid.clone(), gate))):
+        _within(run(), *R.linear(aq, a_s, wq, w_s, b, epi, resid, gate))
+    out = torch.empty((M, 2 * N), dtype=torch.bfloat16, device=cuda)[:, N:]
+    assert mm.apply(x, out=out) is out and torch.equal(out, mm.apply(hip.QuantGroups(*hip.quant_fp8_group128(x))))
+    for name in ("w.weight_scale", "w.weight_scale_inv"):     # a pre-quantised checkpoint loads as it is
+        pre = _plugin("hip-fp8-block128", wq.cpu(), b.cpu(), **{name: w_s.cpu()})
+        pre.to_cuda()
+        assert torch.equal(pre.apply(x), out)
+    assert sorted(pre.state_dict()) == ["w.bias", "w.weight", "w.weight_scale"]
+    # a residual stream in fp32 and a gate per row: the product in bf16, the gated sum as its own pass
+    r32 = resid.float()
+    assert mm.apply_residual_(x, r32, gate) is r32
+    _within(r32, resid.double() + out.double() * gate.double(), 2.0 ** -22 * (resid.double().abs() + (out.double() * gate).abs()))
+    with pytest.raises(hip.Lx2vError):
+        mm.apply(hip.QuantRows(*hip.quant_fp8_rowwise(x)))
+
+
+def test_plugin_fused_members_and_segmented_source(cuda):
+    g = torch.Generator(device=cuda).manual_seed(52)
+    rows, dim = 37, 384
+    x = _rand(g, rows, dim).to(torch.bfloat16)
+    sizes = (256, 128, 72)
+    mods = [_plugin("hip-fp8-block128", _rand(g, n, dim, std=0.05), _rand(g, n) if i != 1 else None) for i, n in enumerate(sizes)]
+    alone = [m.apply(x) for m in mods]
+    fused = type(mods[0]).fused(mods)
+    got = fused.apply(x)
+    slices = [got[:, :256], got[:, 256:384], got[:, 384:]]
+    aq, a_s = hip.quant_fp8_group128(x)
+    for m, a, b in zip(mods, alone, slices):
+        assert m.weight_nk.untyped_storage().data_ptr() == fused.weight_nk.untyped_storage().data_ptr()
+        assert torch.equal(m.apply(x), a)
+        _within(b, *R.linear(aq, a_s, m.weight_nk, m.weight_scale, m.bias))
+    with pytest.raises(ValueError):
+        type(mods[0]).fused([mods[2], mods[0]])
+    parts = x.view(rows, 6, 64).permute(1, 0, 2).contiguous()
+    ks = hip.KSeg(seg=64, stride=rows * 64, split=0, seg2=0, stride2=0, base2=0, lda2=0)
+    a, b = (torch.ones(rows, 256, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    mods[0].apply_residual_(x, a, None)
+    mods[0].apply_residual_(parts[0], b, None, kseg=ks)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("scheme,form", [("hip-fp8-block128", "group"), ("hip-fp8", "row"), ("hip-int8", "int8"), ("hip-bf16", None)])
+def test_residual_norm_plugin_writes_the_form_its_consumers_take(cuda, scheme, form):
+    """x += y, norm, feed-forward, all through the plugins: the norm hands over the 8-bit rows and the Linear takes them as they are."""
+    rows, dim, ffn = 130, 512, 1024
+    g = torch.Generator(device=cuda).manual_seed(53)
+    x, y = _rand(g, rows, dim).to(torch.bfloat16), _rand(g, rows, dim).to(torch.bfloat16)
+    rms = L.RMS_WEIGHT_REGISTER["hip"]("n.weight")
+    rms.load({"n.weight": 1 + 0.1 * _rand(g, dim)})
+    up, down = _plugin(scheme, _rand(g, ffn, dim, std=0.05)), _plugin(scheme, _rand(g, dim, ffn, std=0.05))
+    x2 = x.clone()
+    h = rms.apply_residual_(x2, y, quant_for=up)
+    want = _check_norm(x, y, rms.weight, rms.eps, form)
+    assert type(h) is type(want) and torch.equal(x2, (x.float() + y.float()).to(torch.bfloat16))
+    mid = up.apply_gelu(h)
+    assert torch.equal(mid, up.apply_gelu(want))
+    if form is not None:
+        own = up.apply_gelu(rms.apply_residual_(x.clone(), y))   # quantised by the Linear instead, after a rounding to bf16
+        assert float((own.float() - mid.float()).norm()) <= 2 * 2.0 ** -4 * float(own.float().norm())
+        assert isinstance(rms.apply_residual_(x.clone(), y, quant_for=[up, _plugin("hip-bf16", _rand(g, 8, dim))]), torch.Tensor)   # consumers that differ: bf16
+    down.apply_residual_(mid, x2)
+    assert bool(torch.isfinite(x2.float()).all())
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_wan_block_with_block_scaled_linears(cuda, fused):
+    """The whole block with every Linear block-scaled (both runners) against the fp32 oracle, at the gates of the row-scaled form."""
+    c = case_inputs(load_golden("wan1p3b_g3x6x8"))
+    cfg = {"num_layers": 1, "num_heads": c["heads"], "dim": c["dim"], "task": "t2v", "dit_quant_scheme": "hip-fp8-block128", "fused_block": fused}
+    W = L.WanTransformerWeights(cfg)
+    W.load({k: v.to(cuda) for k, v in {**c["w"], **c["hw"]}.items()})
+    W.to_cuda()
+    inf = L.WanTransformerInfer(cfg)
+    inf.cos_sin = BR.cos_sin_to_real(c["cos_sin"]).contiguous().to(cuda)
+    pre = L.WanPreInferModuleOutput(embed=c["embed"].to(cuda), grid_sizes=c["grid"], x=c["x"].to(torch.bfloat16).to(cuda), embed0=c["embed0"].to(cuda),
+                                    context=c["context"].to(torch.bfloat16).to(cuda))
+    inf.get_scheduler_values = lambda: None
+    out = inf.infer_main_blocks(W.blocks, pre)
+    ref = BR.block_forward(c["x"], c["embed0"], c["context"], c["w"], c["cos_sin"], c["heads"])
+    c_out, c_delta = cos(out, ref), cos(out.float().cpu() - c["x"], ref - c["x"])
+    print(f"\nblock-scaled fp8 block: output cosine {c_out:.6f}, delta cosine {c_delta:.6f}")
+    assert c_out >= 0.999 and c_delta >= 0.99
+
+
+def test_hunyuan_double_block_with_block_scaled_linears(cuda):
+    from tests.test_hy_gpu import HY_CASES, _build, _io
+    from tests.test_hy_oracle import hy_case_inputs
+
+    for name in HY_CASES:
+        rec = load_golden(name)
+        c = hy_case_inputs(rec)
+        W, inf = _build(c, cuda, dit_quant_scheme="hip-fp8-block128")
+        img, txt = inf.infer_double_block(W.double_blocks[0], _io(c, cuda))
+        for got, key, x0 in ((img, "img_out", c["img"]), (txt, "txt_out", c["txt"])):
+            ref = torch.from_numpy(rec[key])
+            assert cos(got[0], ref) >= 0.999 and cos(got[0].float().cpu() - x0[0], ref - x0[0]) >= 0.99, (name, key)

@@ -82,3 +82,33 @@ def test_oracle_quantisation_is_within_half_a_step():
         d = R.dequantise(q, s, rows)
         grid = R.dequantise(torch.ones_like(x).to(torch.float8_e4m3fn), s, rows)
         assert bool(((d - x.double()).abs() <= torch.maximum(2.0 ** -4 * x.double().abs(), 2.0 ** -10 * grid) * (1 + 2.0 ** -20)).all())
+
+
+def test_plugin_is_registered_and_refuses_what_does_not_fit():
+    import lightx2v_amd as L
+
+    cls = L.MM_WEIGHT_REGISTER["hip-fp8-block128"]
+    w = torch.zeros(200, 320).to(torch.float8_e4m3fn)
+    for name in ("w.weight_scale", "w.weight_scale_inv"):
+        mm = cls("w.weight", None)
+        mm.load({"w.weight": w, name: torch.ones(2, 3, dtype=torch.float64)})
+        assert mm.weight_scale.dtype is torch.float32 and mm._calculate_size() == 200 * 320 + 24
+    with pytest.raises(ValueError, match="128 x 128"):    # one scale per output row: another scheme's checkpoint
+        cls("w.weight", None).load({"w.weight": w, "w.weight_scale": torch.ones(200, 1)})
+    with pytest.raises(KeyError):
+        cls("w.weight", None).load({"w.weight": w})
+    with pytest.raises(ValueError, match="fused"):
+        cls.fused([mm, mm])
+    fused = cls.fused([mm])
+    assert fused.weight_nk.shape == (200, 320) and fused.weight_scale.shape == (2, 3)
+    with pytest.raises(ValueError):
+        mm.adopt(w, None)
+    with pytest.raises(NotImplementedError):
+        mm.load_state_dict({}, 0)
+    with pytest.raises(hip.Lx2vError):
+        mm.apply(hip.QuantRows(w, torch.ones(200)))
+    if not torch.cuda.is_available():
+        with pytest.raises(RuntimeError, match="no GPU"):
+            cls("w.weight", None).load({"w.weight": torch.zeros(128, 128)})
+    assert [L.MM_WEIGHT_REGISTER[n].norm_form for n in ("hip-bf16", "hip-fp8", "hip-int8", "hip-fp8-block128")] == [None, "row", "int8", "group"]
+    assert "hip-fp8-block128" in L.WanTransformerWeights({"num_layers": 1, "num_heads": 2, "dim": 256, "task": "t2v", "dit_quant_scheme": "hip-fp8-block128"}).mm_type
