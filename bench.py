@@ -60,6 +60,7 @@ TEXT_DIM = 4096  # umT5-xxl features
 LATENT_CHANNELS = 16
 MFMA_BF16_PEAK_TFLOPS = 2500.0  # dense bf16, MI355X
 MFMA_FP8_PEAK_TFLOPS = 5000.0   # dense fp8 (block-scaled e4m3)
+LINEAR_SCHEMES = {"bf16": "hip-bf16", "fp8": "hip-fp8", "int8": "hip-int8", "fp8-block128": "hip-fp8-block128"}
 ATTN_TYPES = {"bf16": "hip_flash_attn", "fp8": "hip_fp8_attn", "fp8-linear": "hip_fp8_attn_linear"}
 GUIDE_SCALE = 5.0
 
@@ -186,6 +187,7 @@ class KernelClassTimer:
         self.hip, self.enabled, self.rec, self._orig = hip, False, {}, {}
         self._wrap("gemm", "linear_bf16", lambda a, w, *r, **kw: 2.0 * a.shape[0] * w.shape[0] * w.shape[1])
         self._wrap("gemm_fp8", "linear_fp8", lambda a8, a_s, w8, *r, **kw: 2.0 * a8.shape[0] * w8.shape[0] * w8.shape[1])
+        self._wrap("gemm_fp8_block", "linear_fp8", lambda a8, a_s, w8, *r, **kw: 2.0 * a8.shape[0] * w8.shape[0] * w8.shape[1])
         self._wrap("ln_modulate", "norm", lambda x, *r, **kw: float(x.shape[0] * x.shape[1] * (x.element_size() + (1 if kw.get("quant") else 2))))
         self._wrap("rmsnorm_rope", "norm", lambda x, *r, **kw: 4.0 * x.shape[0] * x.shape[1])
         self._wrap("attn_fwd", "attention", lambda q, k, *r, **kw: 4.0 * q.shape[0] * k.shape[0] * q.shape[1] * q.shape[2])
@@ -313,7 +315,7 @@ def arithmetic_label(args):
         return d + " + fp32 residual stream", (suffix[:-1] + ", fp32 residual stream)") if suffix else " (fp32 residual stream)"
     if args.linear == "bf16" and args.attn == "bf16":
         return "bf16", ""
-    lin = {"bf16": "bf16 Linears", "fp8": "fp8 Linears (W8A8 e4m3)", "int8": "int8 Linears (W8A8)"}[args.linear]
+    lin = {"bf16": "bf16 Linears", "fp8": "fp8 Linears (W8A8 e4m3)", "int8": "int8 Linears (W8A8)", "fp8-block128": "fp8 Linears (e4m3, scales per 128)"}[args.linear]
     att = {"bf16": "bf16 attention", "fp8": "fp8 attention (block-scaled e4m3)", "fp8-linear": "fp8 attention (block-scaled e4m3, exp-free P)"}[args.attn]
     return f"{lin} + {att}", " (" + ", ".join(x for x in (f"{args.linear} Linears" if args.linear != "bf16" else "", {"bf16": "", "fp8": "fp8 attention", "fp8-linear": "fp8 attention with exp-free P"}[args.attn]) if x) + ")"
 
@@ -350,7 +352,7 @@ def run_hunyuan(args, dev, world, rank, cfg_p, seq_p, backend, share_gpu, emulat
         seq_group = comm.EmulatedGroup(seq_p)
     C, TEXT_DIM, TXT_TOKENS, BYT5_TOKENS, VIS_TOKENS = 32, 3584, 1000, 256, 729
     cfg = {"mm_double_blocks_depth": layers, "heads_num": H, "hidden_size": D, "task": "t2v", "patch_size": (1, 1, 1), "out_channels": C,
-           "dit_quant_scheme": {"bf16": "hip-bf16", "fp8": "hip-fp8", "int8": "hip-int8"}[args.linear],
+           "dit_quant_scheme": LINEAR_SCHEMES[args.linear],
            "attn_type": ATTN_TYPES[args.attn],
            "seq_parallel": seq_p > 1 or args.sp1, "seq_p_group": seq_group, "parallel": {"seq_p_size": seq_p, "seq_p_attn_type": "hip_ulysses"},
            "enable_cfg": False, "sample_guide_scale": -1.0, "sample_shift": 5.0, "infer_steps": 4, "denoising_step_list": [1000, 750, 500, 250],
@@ -484,8 +486,9 @@ def main():
     ap.add_argument("--res", default=os.environ.get("LX2V_BENCH_RES", "720p"), choices=sorted(GRIDS))
     ap.add_argument("--layout", default=None, help="cfg_p x seq_p, e.g. 2x4 (default: 1x1, 2x1, 2x2, 2x4 for 1/2/4/8 GPUs)")
     ap.add_argument("--layers", type=int, default=None, help="override the layer count (debug only; the JSON line then says so)")
-    ap.add_argument("--linear", default="bf16", choices=["bf16", "fp8", "int8"],
-                    help="arithmetic of the blocks' Linears: bf16 (the headline configuration), W8A8 e4m3 (the reference's fp8 schemes) or W8A8 int8 (its int8 schemes)")
+    ap.add_argument("--linear", default="bf16", choices=list(LINEAR_SCHEMES),
+                    help="arithmetic of the blocks' Linears: bf16 (the headline configuration), W8A8 e4m3 (the reference's fp8 schemes), W8A8 int8 (its int8 schemes) "
+                         "or e4m3 with a scale per 128 columns / 128 x 128 block (its per-block-128 scheme)")
     ap.add_argument("--attn", default="bf16", choices=["bf16", "fp8", "fp8-linear"],
                     help="self-attention arithmetic: bf16 (the headline configuration), block-scaled e4m3 on the fp8 MFMA (where the reference would run a quantised backend), "
                          "or the same with P taken as 2^x with a linear mantissa instead of by exps")
@@ -611,7 +614,7 @@ def main():
     cfg = {"num_layers": layers, "num_heads": H, "dim": D, "ffn_dim": F, "task": "t2v", "model_cls": "wan2.1",
            "in_dim": LATENT_CHANNELS, "out_dim": LATENT_CHANNELS, "freq_dim": 256, "infer_steps": 50, "sample_shift": 5.0,
            "sample_guide_scale": GUIDE_SCALE, "enable_cfg": True, "run_device": "cuda",
-           "dit_quant_scheme": {"bf16": "hip-bf16", "fp8": "hip-fp8", "int8": "hip-int8"}[args.linear],
+           "dit_quant_scheme": LINEAR_SCHEMES[args.linear],
            "self_attn_1_type": ATTN_TYPES[args.attn],
            "sensitive_layer_dtype": "fp32" if args.residual == "fp32" else "bf16",
            "cfg_parallel": cfg_p > 1, "cfg_p_group": cfg_group,
