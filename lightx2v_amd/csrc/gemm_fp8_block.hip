@@ -59,12 +59,13 @@ LX2V_DEVICE void static_for(F&& f) {
   }
 }
 
-LX2V_DEVICE u32x4 raw_descriptor(const void* base, int64_t bytes) {
+// (an operand tile of at most 256 rows, each below 8 MiB: the extent is below 2^31 and computed in 32 bits)
+LX2V_DEVICE u32x4 raw_descriptor(const void* base, uint32_t bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(base);
   u32x4 d;
   d[0] = __builtin_amdgcn_readfirstlane((uint32_t)a);
   d[1] = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));  // stride 0: raw buffer
-  d[2] = __builtin_amdgcn_readfirstlane((uint32_t)(bytes < 0 ? 0 : (bytes > 0x7fffffffLL ? 0x7fffffffLL : bytes)));  // loads at or past it return 0
+  d[2] = __builtin_amdgcn_readfirstlane(bytes);  // loads at or past it return 0
   d[3] = 0x00020000u;
   return d;
 }
@@ -209,7 +210,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   const Raster raster{p.tiles_m, p.tiles_n, ntiles >> 3, ntiles & 7, p.group_rcp};
   const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t)(size_t)(__attribute__((address_space(3))) char*)lds);
   constexpr int NOWHERE = (int)0x80000000u;
-  const bool sw_wave = wid == 3, sa_wave = wid < (T::TM + 63) / 64;
+  const bool sw_wave = wid == 3;  // (waves 0 - 2: 64 rows' scales each; past the tile's rows they read zeros)
 
   // ---- DMA cursors: W and its scales SW blocks ahead of the multiplied one, A SA blocks ----
   // piece q of wave w: rows 32 q + 8 w + (lane >> 3) of the operand tile; the swizzle is the same for all q
@@ -218,15 +219,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   const int ragged = left < BK && kb0 + nk == p.nk ? nk - 1 : -1;
   int a_pv, w_pv, s_pv = NOWHERE;
   auto offset = [&](int64_t ld, bool last) __attribute__((always_inline)) -> int {  // of piece 0; `last`: chunks past K go nowhere
-    return last && chunk * 16 >= left ? NOWHERE : (8 * wid + (lane >> 3)) * (int)ld + chunk * 16;
+    int at = (8 * wid + (lane >> 3)) * (int)ld + chunk * 16;
+    asm volatile("" : "+v"(at));  // (a branch around it would make the scalars that meet behind it vector registers)
+    return last & (chunk * 16 >= left) ? NOWHERE : at;
   };
   struct Cursor {
     int ord = 0, kt = 0;
     uint32_t soff = 0;
   } ca, cw;
-  u32x4 a_rs, w_rs, s_rs;
-  // the scales' descriptor moves on by a block's scales: 64-bit base, the same extent
-  uint64_t s_base = 0, s_step = 0;
+  u32x4 a_rs, w_rs;
+  uint64_t s_base = 0, s_step = 0;  // the scales' descriptor: its base moves on by a block's scales, its extent stays
+  uint32_t s_bytes = 0;
   // (the fields are read together: one wait for memory per tile and operand, not one for each field on its first use)
   auto a_tile = [&]() __attribute__((always_inline)) {  // descriptor of the cursor's output tile; past the last one it is empty
     const ParamsAgain p = params_again();
@@ -238,7 +241,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     int m0, n0;
     tile_origin(raster, vbid, T::TM, T::TN, m0, n0);
     const int rows = vbid < ntiles ? min(M - m0, T::TM) : 0;
-    a_rs = raw_descriptor(reinterpret_cast<const uint8_t*>(base) + (int64_t)(rows ? m0 : 0) * lda, (int64_t)rows * lda);
+    a_rs = raw_descriptor(reinterpret_cast<const uint8_t*>(base) + (int64_t)(rows ? m0 : 0) * lda, (uint32_t)rows * (uint32_t)lda);
+    asm volatile("" : "+s"(a_rs));
   };
   auto w_tile = [&]() __attribute__((always_inline)) {
     const ParamsAgain p = params_again();
@@ -252,11 +256,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     tile_origin(raster, vbid, T::TM, T::TN, m0, n0);
     if (!live) m0 = n0 = 0;
     const int rows = live ? min(N - n0, T::TN) : 0;
-    w_rs = raw_descriptor(reinterpret_cast<const uint8_t*>(base) + (int64_t)n0 * ldw, (int64_t)rows * ldw);
+    w_rs = raw_descriptor(reinterpret_cast<const uint8_t*>(base) + (int64_t)n0 * ldw, (uint32_t)rows * (uint32_t)ldw);
     const int nb = min(((N + 127) >> 7) - (n0 >> 7), (T::TN + 127) / 128);  // weight row blocks of the tile
     const float* sb = sw_wave ? reinterpret_cast<const float*>(wsb) + (int64_t)(n0 >> 7) * lds_w + kb0 : reinterpret_cast<const float*>(asb) + (int64_t)kb0 * lds_a + m0;
-    s_rs = raw_descriptor(sb, !live ? 0 : sw_wave ? ((int64_t)(nb - 1) * lds_w + 1) * 4 : sa_wave ? ((int64_t)M - m0) * 4 : 0);
-    s_base = ((uint64_t)s_rs[1] << 32) | s_rs[0];
+    s_base = reinterpret_cast<uint64_t>(sb);
+    s_bytes = !live ? 0u : sw_wave ? ((uint32_t)(nb - 1) * (uint32_t)lds_w + 1) * 4 : (uint32_t)min(M - m0, T::TM) * 4;
+    asm volatile("" : "+s"(w_rs), "+s"(s_base), "+s"(s_bytes));
     s_pv = sw_wave ? (lane < nb ? lane * (int)lds_w * 4 : NOWHERE) : (64 * wid + lane) * 4;
   };
   a_tile();
@@ -268,15 +273,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     const int64_t step = sw_wave ? 4 : p.lds_a * 4;
     s_step = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)step >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)step);
   }
-  uint32_t dma_base = lds_base + 1024 * (uint32_t)wid, dma_sc = lds_base + 256 * (uint32_t)wid;
+  uint32_t dma_base = lds_base + 1024 * (uint32_t)wid, dma_sc;
+  asm volatile("" : "+s"(dma_base));
+  dma_sc = lds_base + ((dma_base - lds_base) >> 2);
+  asm volatile("" : "+s"(dma_sc));
   auto set_m0 = [&](uint32_t base, auto ofsc) __attribute__((always_inline)) { asm volatile("s_add_u32 m0, %0, %1" ::"s"(base), "i"(decltype(ofsc)::value) : "memory", "scc"); };
   auto load16 = [&](const u32x4& rs, int voff, uint32_t soff) __attribute__((always_inline)) {
     asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(rs), "s"(soff) : "memory");
   };
-  auto load4 = [&](const u32x4& rs, int voff) __attribute__((always_inline)) { asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rs) : "memory"); };
+  auto load4 = [&]() __attribute__((always_inline)) {  // (the descriptor is put together here: as a vector that lives on, the compiler moves it into vector registers)
+    asm volatile("s_mov_b64 s[96:97], %1\n\ts_mov_b32 s98, %2\n\ts_mov_b32 s99, 0x20000\n\tbuffer_load_dword %0, s[96:99], 0 offen lds"
+                 ::"v"(s_pv), "s"(s_base), "s"(s_bytes) : "memory", "s96", "s97", "s98", "s99");
+  };
   // Ring positions: of block j, which the DMA refills, and of block j + 1, which is read.  (Two W slots: W and the scales of block j
   // lie at the parity P of j, known at compile time.)
   uint32_t a_cur = dma_base, a_nxt = dma_base + T::A_BYTES, w_cur = dma_base, w_nxt = dma_base + T::W_BYTES, s_cur = dma_sc, s_nxt = dma_sc + 1024;
+  asm volatile("" : "+s"(a_cur), "+s"(a_nxt), "+s"(w_cur), "+s"(w_nxt), "+s"(s_cur), "+s"(s_nxt));
   constexpr bool TWO = T::SW == 2;
   // piece q of a block's DMA, its target and then the load itself: W(j + SW), its scales, A(j + SA)
   auto dma_set = [&](auto Pc, auto qc) __attribute__((always_inline)) {
@@ -294,7 +306,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       load16(w_rs, d_voff, cw.soff);
       if constexpr (q + 1 < T::PW) d_voff += w_step;
     } else if constexpr (q == T::PW) {
-      load4(s_rs, s_pv);
+      load4();
     } else {
       if constexpr (q == T::PW + 1) d_voff = a_pv;
       load16(a_rs, d_voff, ca.soff);
@@ -302,12 +314,33 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     }
     asm volatile("" : "+v"(d_voff));
   };
-  auto w_advance = [&]() __attribute__((always_inline)) {
-    ++cw.kt;
-    cw.soff += BK;
-    s_base += s_step;
-    s_rs[0] = (uint32_t)s_base;
-    s_rs[1] = (uint32_t)(s_base >> 32);
+  // Cursors and rings move on by a block: four pieces of a few scalar instructions, W's (0 - 2) once its DMA of the block is issued,
+  // then A's; what the end of a tile needs besides follows in w_turn and a_turn.
+  constexpr int MOVES = 4;
+  auto move = [&](auto ic) __attribute__((always_inline)) {
+    constexpr int i = decltype(ic)::value;
+    if constexpr (i == 0) {
+      ++cw.kt;
+      cw.soff += BK;
+      s_base += s_step;
+      asm volatile("" : "+s"(cw.kt), "+s"(cw.soff), "+s"(s_base));
+    } else if constexpr (i == 1 && !TWO) {
+      w_cur = w_nxt;
+      w_nxt = w_nxt == dma_base + (T::SW - 1) * T::W_BYTES ? dma_base : w_nxt + T::W_BYTES;
+      asm volatile("" : "+s"(w_cur), "+s"(w_nxt));
+    } else if constexpr (i == 2 && !TWO) {
+      s_cur = s_nxt;
+      s_nxt = s_nxt == dma_sc + (T::SW - 1) * 1024 ? dma_sc : s_nxt + 1024;
+      asm volatile("" : "+s"(s_cur), "+s"(s_nxt));
+    } else if constexpr (i == 3) {
+      ++ca.kt;
+      ca.soff += BK;
+      a_cur = a_nxt;
+      a_nxt = a_nxt == dma_base + (T::SA - 1) * T::A_BYTES ? dma_base : a_nxt + T::A_BYTES;
+      asm volatile("" : "+s"(ca.kt), "+s"(ca.soff), "+s"(a_cur), "+s"(a_nxt));
+    }
+  };
+  auto w_turn = [&]() __attribute__((always_inline)) {
     if (cw.kt == ragged) w_pv = offset(params_again()->ldw, true);
     if (cw.kt == nk) {
       cw.kt = 0;
@@ -316,18 +349,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       w_tile();
       if (ragged >= 0) w_pv = offset(params_again()->ldw, ragged == 0);
     }
-    if constexpr (!TWO) {
-      w_cur = w_nxt;
-      w_nxt = w_nxt == dma_base + (T::SW - 1) * T::W_BYTES ? dma_base : w_nxt + T::W_BYTES;
-      s_cur = s_nxt;
-      s_nxt = s_nxt == dma_sc + (T::SW - 1) * 1024 ? dma_sc : s_nxt + 1024;
-      asm volatile("" : "+s"(w_cur), "+s"(w_nxt), "+s"(s_cur), "+s"(s_nxt));
-    }
-    asm volatile("" : "+s"(w_rs), "+s"(s_rs), "+s"(s_base), "+s"(cw.soff), "+s"(cw.kt), "+s"(cw.ord), "+s"(dma_base), "+s"(dma_sc));
+    asm volatile("" : "+s"(w_rs), "+s"(s_base), "+s"(s_bytes), "+s"(cw.soff), "+s"(cw.kt), "+s"(cw.ord), "+s"(dma_base), "+s"(dma_sc));
   };
-  auto a_advance = [&]() __attribute__((always_inline)) {
-    ++ca.kt;
-    ca.soff += BK;
+  auto a_turn = [&]() __attribute__((always_inline)) {
     if (ca.kt == ragged) a_pv = offset(params_again()->lda, true);
     if (ca.kt == nk) {
       ca.kt = 0;
@@ -336,8 +360,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       a_tile();
       if (ragged >= 0) a_pv = offset(params_again()->lda, ragged == 0);
     }
-    a_cur = a_nxt;
-    a_nxt = a_nxt == dma_base + (T::SA - 1) * T::A_BYTES ? dma_base : a_nxt + T::A_BYTES;
     asm volatile("" : "+s"(a_rs), "+s"(ca.soff), "+s"(ca.kt), "+s"(ca.ord), "+s"(a_cur), "+s"(a_nxt));
   };
 
@@ -419,13 +441,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
           static_for<r, r + 2>([&](auto rc) __attribute__((always_inline)) { rd(IntC<Q>{}, rc); });
         }
       } else {  // few MFMAs: pieces spread over the steps, reads over the first three quarters of them
-        static_for<t * T::PIECES / T::STEPS, (t + 1) * T::PIECES / T::STEPS>([&](auto qc) __attribute__((always_inline)) {
+        constexpr int D = T::STEPS - 1, q0 = t * T::PIECES / D, q1 = (t + 1) * T::PIECES / D;  // (none in the last step: A moves on there)
+        static_for<(q0 < T::PIECES ? q0 : T::PIECES), (q1 < T::PIECES ? q1 : T::PIECES)>([&](auto qc) __attribute__((always_inline)) {
           dma_set(IntC<P>{}, qc);
           asm volatile("s_nop 0");
           dma_go(qc);
         });
         constexpr int E = T::STEPS * 3 / 4, r0 = t * T::READS / E, r1 = (t + 1) * T::READS / E;
         static_for<(r0 < T::READS ? r0 : T::READS), (r1 < T::READS ? r1 : T::READS)>([&](auto rc) __attribute__((always_inline)) { rd(IntC<Q>{}, rc); });
+      }
+      if constexpr (T::STEPS == 8) {
+        if constexpr (t >= 5) static_for<t - 5, (t == 7 ? MOVES : t - 4)>(move);
+      } else if constexpr (t >= T::STEPS - MOVES) {
+        move(IntC<t - (T::STEPS - MOVES)>{});
       }
       __builtin_amdgcn_sched_barrier(0);
       constexpr int last = T::STEPS - 2 + t;
@@ -450,7 +478,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     int fr_ = fr, fq_ = fq;
     asm volatile("" : "+v"(fr_), "+v"(fq_));
     if constexpr (EPI == EPI_PARTIAL) {
-      const u32x4 d = raw_descriptor(p->partials + ((int64_t)part_id * M + m0) * N, (int64_t)min(M - m0, T::TM) * N * 4);
+      const u32x4 d = raw_descriptor(p->partials + ((int64_t)part_id * M + m0) * N, (uint32_t)min(M - m0, T::TM) * (uint32_t)N * 4);
       const auto o_rs = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)d[1] << 32) | d[0]), 0, (int)d[2], 0x00020000);
       static_for<0, MT * NT>([&](auto uc) __attribute__((always_inline)) {
         constexpr int i = decltype(uc)::value / NT, k = decltype(uc)::value % NT;
@@ -459,14 +487,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       });
       return;
     }
-    auto resource = [](uint64_t at, int64_t bytes) __attribute__((always_inline)) {  // accesses past the end: loads give 0, stores are dropped
+    auto resource = [](uint64_t at, uint32_t bytes) __attribute__((always_inline)) {  // accesses past the end: loads give 0, stores are dropped
       const u32x4 d = raw_descriptor(reinterpret_cast<const void*>(at), bytes);
       return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)d[1] << 32) | d[0]), 0, (int)d[2], 0x00020000);
     };
-    const int64_t rows = min(M - m0, T::TM);
-    const auto c_rs = resource(c_at + (int64_t)m0 * ldc * 2, (rows - 1) * ldc * 2 + (int64_t)N * 2);
-    const auto r_rs = resource(resid_at + (int64_t)m0 * ldr * 2, EPI == LX2V_EPI_RESIDUAL ? (rows - 1) * ldr * 2 + (int64_t)N * 2 : 0);
-    const auto b_rs = resource(bias_at, bias_at ? (int64_t)N * 4 : 0), g_rs = resource(gate_at, EPI == LX2V_EPI_RESIDUAL && gate_at ? (int64_t)N * 4 : 0);
+    const uint32_t rows = (uint32_t)min(M - m0, T::TM);
+    const auto c_rs = resource(c_at + (int64_t)m0 * ldc * 2, ((rows - 1) * (uint32_t)ldc + (uint32_t)N) * 2);
+    const auto r_rs = resource(resid_at + (int64_t)m0 * ldr * 2, EPI == LX2V_EPI_RESIDUAL ? ((rows - 1) * (uint32_t)ldr + (uint32_t)N) * 2 : 0);
+    const auto b_rs = resource(bias_at, bias_at ? (uint32_t)N * 4 : 0), g_rs = resource(gate_at, EPI == LX2V_EPI_RESIDUAL && gate_at ? (uint32_t)N * 4 : 0);
     // step u = column block pair u / MT, row block u % MT.  Bias and gate are loaded one pair ahead, residual rows RV steps ahead.
     // (the residual form has registers for one pair's bias and gate only)
     constexpr int U = MT * NT / 2, RV = MT, CV = EPI == LX2V_EPI_RESIDUAL ? 1 : 2;
@@ -551,8 +579,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       asm volatile("s_nop 0");
       dma_go(qc);
     });
-    if constexpr (b < T::SW) w_advance();
-    a_advance();
+    static_for<(b < T::SW ? 0 : 3), MOVES>(move);
+    if constexpr (b < T::SW) w_turn();
+    a_turn();
   });
   // (the rings are back at slot 0: block 0's)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -566,8 +595,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   auto step = [&](auto Pc) __attribute__((always_inline)) {
     if (kt == 0) block(Pc, IntC<1>{}, relaxed);
     else block(Pc, IntC<0>{}, false);
-    w_advance();
-    a_advance();
+    if (max(cw.kt, ca.kt) >= nk - 1) {
+      w_turn();
+      a_turn();
+    }
     relaxed = false;
     if (++kt == nk) {
       int m0, n0;
