@@ -109,7 +109,7 @@ LX2V_DEVICE void finish4(const Params& p, const f32x4& acc, int64_t m, int n) {
 // walks its output tiles as one stream of K blocks.  Block j is multiplied while block j + 1 is read from LDS into the other
 // set of fragment registers (so the LDS reads are spread over the whole block) and the blocks behind it are on their way into
 // rings of SA A slots and SW W slots: once every wave has block j in registers, its slots take W(j + SW) with its scales and
-// A(j + SA).  (192 x 256, at 75600 x 5120 x 13824 with the gated residual: 4.6 ms = 2.3 PFLOP/s.  The MFMAs are busy 65 % of the
+// A(j + SA).  (192 x 256, at 75600 x 5120 x 13824 with the gated residual: 4.5 ms = 2.4 PFLOP/s.  The MFMAs are busy 66 % of the
 // cycles at a clock that sinks to 1.6 GHz under them; two A slots instead of three: 5.0 ms; the first version, which read its
 // fragments after the barrier: 8 ms.)
 // LDS: a row's eight 16-byte chunks c lie at c ^ ((row >> 1) & 7).  A lane takes chunks fq and fq + 4 of its row as the two halves of a
@@ -736,14 +736,17 @@ struct Plan {
 };
 
 // Up to 32 rows the skinny kernel (13 x 5120 x 4096: 9.4 us, the 64 x 128 tile split four ways 12.6; 32 x 5120 x 5120: 12.4 and 14.5;
-// at 64 rows its reads of A cost more than they save, 17.4 and 15.5).  Above, the kernel and split whose estimated time is least.  A tile kernel's time is rounds of one tile (or K range) per CU, each a number
-// of K blocks and an overhead (pipeline fill, epilogue, tile switch); measured on this hardware, one workgroup per CU:
+// at 64 rows its reads of A cost more than they save, 17.4 and 15.2).  Above, the kernel and split whose estimated time is least.
+// A tile kernel's time is rounds of tiles, each of K blocks and an overhead (pipeline fill, epilogue, tile switch); measured with
+// one tile on nearly every CU, K = 2560 and 10240:
 //   tile        us per K block   us per tile
-//   192 x 256        1.15             5          (one wave's 48 MFMAs are 0.64 us at 2.4 GHz; the rest is memory latency and clock)
-//   128 x 256        0.85             4
-//   128 x 128        0.60             3
-//   64 x 128         0.50             2
+//   192 x 256        1.08            10          (one wave's 48 MFMAs are 0.64 us at 2.4 GHz; the CU's LDS moves 168 KB meanwhile)
+//   128 x 256        0.84             8
+//   128 x 128        0.55             5
+//   64 x 128         0.41             3
 // A split along K adds a launch that reads the partial sums back: 5 us and their bytes, written and read, at 4 TB/s.
+// (512 x 10240 x 5120: 128 x 256 whole 35.7 us, 192 x 256 44.9, 128 x 128 47.6; 2500 x 1536 x 8960: 128 x 128 whole 43.1,
+// 128 x 256 in two parts 46.4; 64 x 5120 x 5120: 64 x 128 in four parts 15.2, whole 20.2; 200 x 5120 x 13824: in three 29.5, 43.9.)
 Plan make_plan(int64_t M, int64_t N, int64_t K, int cus) {
   const int nk = (int)((K + BK - 1) / BK);
   if (M <= 16) return Plan{SKINNY_16, 16, 16, 1, nk, 0};
@@ -752,7 +755,7 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int cus) {
     Kind kind;
     int tm, tn;
     float block, tile;
-  } kinds[] = {{TILE_192x256, 192, 256, 1.15f, 5.f}, {TILE_128x256, 128, 256, 0.85f, 4.f}, {TILE_128x128, 128, 128, 0.60f, 3.f}, {TILE_64x128, 64, 128, 0.50f, 2.f}};
+  } kinds[] = {{TILE_192x256, 192, 256, 1.08f, 10.f}, {TILE_128x256, 128, 256, 0.84f, 8.f}, {TILE_128x128, 128, 128, 0.55f, 5.f}, {TILE_64x128, 64, 128, 0.41f, 3.f}};
   Plan best{TILE_192x256, 192, 256, 1, nk, 0};
   float least = 1e30f;
   for (const auto& k : kinds) {

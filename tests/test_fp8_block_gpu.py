@@ -36,7 +36,8 @@ SHAPES = [(1, 8, 16), (1, 64, 128), (1, 5120, 5120), (2, 136, 112), (13, 520, 14
           (200, 384, 640), (257, 5120, 1280), (512, 1536, 8960), (1000, 2056, 1456), (1111, 4096, 384), (4100, 3080, 208), (9000, 1544, 528), (193, 13824, 5120),
           # each tile kernel with one block of K and with two, one tile and several for a workgroup; split along K with a ragged last part
           (70, 136, 16), (900, 1288, 96), (12001, 136, 16), (577, 4104, 144), (20000, 520, 16), (20000, 520, 144), (12001, 1288, 16), (12001, 1288, 144), (20000, 776, 1040),
-          (40, 512, 2048), (70, 136, 4112), (70, 8200, 4112), (484, 4096, 8976), (151, 8960, 13840)]
+          (40, 512, 2048), (70, 136, 4112), (70, 8200, 4112), (484, 4096, 8976), (151, 8960, 13840),
+          (385, 8200, 16), (385, 8200, 272), (77, 5120, 13840), (262, 4096, 13840), (151, 8960, 16400)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
