@@ -779,7 +779,7 @@ class QuantGroups(QuantRows):
 
 def _launch(entry: str, device: int, *args):
     """Call an entry point on the current stream of the operands' device (which need not be the current device)."""
-    if device == torch.cuda.current_device():
+    if device == torch._C._cuda_getDevice():  # (torch.cuda.current_device without its check for an initialised GPU, which holds the operands)
         st = getattr(load(), entry)(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
@@ -809,12 +809,13 @@ def _dense_vec(name: str, t: Optional[torch.Tensor], n: int, like: torch.Tensor)
 
 def _row_stride(t: torch.Tensor) -> int:
     """Row stride as the C ABI wants it: of a tensor with at most one row torch may report anything."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), (t.shape[1] + 15) // 16 * 16)
+    rows, dim = t.shape
+    return t.stride(0) if rows > 1 else dim + 15 & ~15
 
 
 def _group_scales(rows: int, dim: int, device) -> torch.Tensor:
-    """Uninitialised fp32 scales in memory order, [groups, rows]; the transposed view is QuantGroups' layout."""
-    return torch.empty(((dim + BLOCK - 1) // BLOCK, rows), dtype=torch.float32, device=device)
+    """Uninitialised fp32 scales [rows, groups] of QuantGroups, stored group after group."""
+    return torch.empty_strided((rows, (dim + BLOCK - 1) // BLOCK), (1, rows), dtype=torch.float32, device=device)
 
 
 def _group_stride(scale: torch.Tensor) -> int:
@@ -837,7 +838,7 @@ def quant_fp8_group128(x: torch.Tensor, kseg: Optional["KSeg"] = None, dim: Opti
         _launch("lx2v_quant_fp8_group128_f32", device.index, x.data_ptr(), _row_stride(x), q.data_ptr(), dim, scale.data_ptr(), max(rows, 1), rows, dim)
     else:
         _launch("lx2v_quant_fp8_group128", device.index, x.data_ptr(), _row_stride(x), None if kseg is None else ctypes.byref(kseg), q.data_ptr(), dim, scale.data_ptr(), max(rows, 1), rows, dim)
-    return q, scale.t()
+    return q, scale
 
 
 def quant_fp8_block128(w: torch.Tensor):
@@ -944,4 +945,4 @@ def add_rmsnorm_(x: torch.Tensor, y: Optional[torch.Tensor], weight=None, eps: f
     scale = _group_scales(rows, dim, device) if quant == "group" else torch.empty((rows,), dtype=torch.float32, device=device)
     _launch("lx2v_add_rmsnorm_quant_f32" if f32 else "lx2v_add_rmsnorm_quant_bf16", device.index, *args, q.data_ptr(), dim, scale.data_ptr(),
             max(rows, 1) if quant == "group" else 0, _NORM_FORMS[quant], rows, dim, eps)
-    return QuantGroups(q, scale.t()) if quant == "group" else QuantRows(q, scale)
+    return QuantGroups(q, scale) if quant == "group" else QuantRows(q, scale)
