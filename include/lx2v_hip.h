@@ -450,7 +450,7 @@ int lx2v_gemm_fp8_block128(const uint8_t* A, int64_t lda, const float* a_scale, 
  * The residual addition of a pre-norm layer and the RMSNorm behind it in one pass (over the whole row, as
  * lx2v_rmsnorm_rope_bf16 with do_norm = 1).  x: the residual stream, bf16 or fp32 rows; y bf16 rows, or NULL (nothing is
  * added and x is only read); w fp32 [dim] or NULL.  The norm sees the fp32 sum, before it is rounded to x's type.
- * `out` may alias y, not x.  dim % 8 == 0, dim <= 8192.
+ * `out` may alias y, not x.  dim % 8 == 0, dim <= 8192.  rows < 2^24 (2^26 up to 1024 columns).
  * The _quant forms leave the normalised row in 8 bits, rounded once from fp32: `form`
  *   LX2V_QUANT_FP8_ROW      e4m3, scale[r], the rule of lx2v_quant_fp8_rowwise      (operand of lx2v_gemm_fp8)
  *   LX2V_QUANT_FP8_GROUP128 e4m3, scale[g * ld_scale + r] per 128 columns           (operand of lx2v_gemm_fp8_block128)

@@ -109,9 +109,9 @@ LX2V_DEVICE void finish4(const Params& p, const f32x4& acc, int64_t m, int n) {
 // walks its output tiles as one stream of K blocks.  Block j is multiplied while block j + 1 is read from LDS into the other
 // set of fragment registers (so the LDS reads are spread over the whole block) and the blocks behind it are on their way into
 // rings of SA A slots and SW W slots: once every wave has block j in registers, its slots take W(j + SW) with its scales and
-// A(j + SA).  (192 x 256, at 75600 x 5120 x 13824 with the gated residual: 4.5 ms = 2.4 PFLOP/s.  The MFMAs are busy 66 % of the
-// cycles at a clock that sinks to 1.6 GHz under them; two A slots instead of three: 5.0 ms; the first version, which read its
-// fragments after the barrier: 8 ms.)
+// A(j + SA).  (192 x 256, at 75600 x 5120 x 13824 with the gated residual: 4.5 ms = 2.4 PFLOP/s.  The MFMAs are busy 69 % of the
+// cycles at a clock that sinks to 1.6 GHz under them; two A slots instead of three: 5.0 ms; eight waves and one set of fragment
+// registers: 10.3 ms.)
 // LDS: a row's eight 16-byte chunks c lie at c ^ ((row >> 1) & 7).  A lane takes chunks fq and fq + 4 of its row as the two halves of a
 // fragment instead of 2 fq and 2 fq + 1 -- any order of K that both operands share gives the same products -- because the LDS serves
 // the lanes of a 16-byte read in eights out of two neighbouring quarters, and so all eight hit different banks (counter: no conflicts).

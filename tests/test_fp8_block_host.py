@@ -58,6 +58,10 @@ def test_quantisers_and_norm_refuse(p):
     assert lib.lx2v_add_rmsnorm_bf16(p, 64, p, 64, None, p + 64, 64, 4, 60, 1e-6, None) == -2
     assert lib.lx2v_add_rmsnorm_f32(p, 64, p, 56, None, p + 64, 64, 4, 64, 1e-6, None) == -1
     assert lib.lx2v_add_rmsnorm_f32(p, 64, p, 64, p + 4, p + 64, 64, 4, 64, 1e-6, None) == -1
+    # more workgroups than a launch has
+    assert lib.lx2v_add_rmsnorm_bf16(p, 2048, p, 2048, None, p + 64, 2048, 1 << 24, 2048, 1e-6, None) == -2 and b"workgroups" in lib.lx2v_last_error()
+    assert lib.lx2v_add_rmsnorm_f32(p, 64, p, 64, None, p + 64, 64, 1 << 26, 64, 1e-6, None) == -2
+    assert lib.lx2v_quant_fp8_group128(p, 512, None, p, 512, p, 1 << 29, 1 << 29, 512, None) == -2 and b"workgroups" in lib.lx2v_last_error()
     for form in (-1, 3):
         assert lib.lx2v_add_rmsnorm_quant_bf16(p, 64, p, 64, None, p + 64, 64, p, 4, form, 4, 64, 1e-6, None) == -1 and b"form" in lib.lx2v_last_error()
     assert lib.lx2v_add_rmsnorm_quant_bf16(p, 64, p, 64, None, p + 64, 64, None, 4, 0, 4, 64, 1e-6, None) == -1
