@@ -175,20 +175,41 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(T* x, int64_t ldx, con
   T* xr = x + row * ldx;
   float f[NC][8];
   float ss = 0.f;
+  // As in the group quantiser: short calls load without branches in between (lanes past the row's end its last chunk again; one row
+  // of 5120 3.3 us against 3.7, [4680, 5120] 32.2 against 34.0), long ones chunk by chunk ([75600, 5120] 481 against 491).
+  if constexpr (BIG) {
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int ch = t + TPR * c;
+    for (int c = 0; c < NC; ++c) {
+      const int ch = t + TPR * c;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[c][j] = 0.f;
-    if (ch < nchunks) {
-      load8_once<BIG>(xr + ch * 8, f[c]);
-      if (y != nullptr) {
-        float b[8];
-        load8_once<BIG>(y + row * ldy + ch * 8, b);
+      for (int j = 0; j < 8; ++j) f[c][j] = 0.f;
+      if (ch < nchunks) {
+        load8_once<BIG>(xr + ch * 8, f[c]);
+        if (y != nullptr) {
+          float b[8];
+          load8_once<BIG>(y + row * ldy + ch * 8, b);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[c][j] += b[j];
+          for (int j = 0; j < 8; ++j) f[c][j] += b[j];
+        }
       }
     }
+  } else {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) load8_once<BIG>(xr + min(t + TPR * c, nchunks - 1) * 8, f[c]);
+    if (y != nullptr) {
+      const uint16_t* yr = y + row * ldy;
+      float b[NC][8];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) load8_once<BIG>(yr + min(t + TPR * c, nchunks - 1) * 8, b[c]);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[c][j] += b[c][j];
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[c][j] = t + TPR * c < nchunks ? f[c][j] : 0.f;
   }
 #pragma unroll
   for (int c = 0; c < NC; ++c)
