@@ -866,23 +866,27 @@ def gemm_fp8_block(a8: torch.Tensor, a_scale: torch.Tensor, w8: torch.Tensor, w_
     calls that share one must be ordered on one stream); absent, it comes from torch's allocator when one is needed."""
     f8, f32 = torch.float8_e4m3fn, torch.float32
     dev = a8.get_device()   # -1: not a GPU tensor
-    for n, t in (("a8", a8), ("w8", w8)):
-        if dev < 0 or t.get_device() != dev or t.dtype is not f8 or t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
-            raise Lx2vError(f"gemm_fp8_block: {n} must be a float8_e4m3fn matrix on one GPU with a contiguous inner dimension, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if dev < 0 or w8.get_device() != dev or a8.dtype is not f8 or w8.dtype is not f8 or a8.dim() != 2 or w8.dim() != 2 or a8.stride(1) != 1 or w8.stride(1) != 1:
+        raise Lx2vError("gemm_fp8_block: a8 and w8 must be float8_e4m3fn matrices on one GPU with a contiguous inner dimension, got "
+                        + " and ".join(f"{t.dtype} {tuple(t.shape)} stride {t.stride()} on {t.device}" for t in (a8, w8)))
     M, K = a8.shape
     N, kw = w8.shape
     if kw != K:
         raise Lx2vError(f"gemm_fp8_block: K mismatch {K} vs {kw}")
     groups = (K + BLOCK - 1) // BLOCK
-    for n, t, shape in (("a_scale", a_scale, (M, groups)), ("w_scale", w_scale, ((N + BLOCK - 1) // BLOCK, groups))):
-        if t.get_device() != dev or t.dtype is not f32 or t.shape != shape:
-            raise Lx2vError(f"gemm_fp8_block: {n} must be fp32 {shape} on {a8.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    blocks = (N + BLOCK - 1) // BLOCK
+    if (a_scale.shape != (M, groups) or w_scale.shape != (blocks, groups) or a_scale.dtype is not f32 or w_scale.dtype is not f32 or a_scale.get_device() != dev
+            or w_scale.get_device() != dev):
+        raise Lx2vError(f"gemm_fp8_block: a_scale must be fp32 {(M, groups)} and w_scale fp32 {(blocks, groups)} on {a8.device}, got "
+                        + " and ".join(f"{t.dtype} {tuple(t.shape)} on {t.device}" for t in (a_scale, w_scale)))
     if (M > 1 and a_scale.stride(0) != 1) or (groups > 1 and a_scale.stride(1) < M):
         a_scale = a_scale.t().contiguous().t()
     if not w_scale.is_contiguous():
         w_scale = w_scale.contiguous()
-    bias = _dense_vec("gemm_fp8_block.bias", bias, N, a8)
-    gate = _dense_vec("gemm_fp8_block.gate", gate, N, a8)
+    if bias is not None:
+        bias = _dense_vec("gemm_fp8_block.bias", bias, N, a8)
+    if gate is not None:
+        gate = _dense_vec("gemm_fp8_block.gate", gate, N, a8)
     if out is None:
         out = torch.empty((M, N), dtype=torch.bfloat16, device=a8.device)
         ldc = N
