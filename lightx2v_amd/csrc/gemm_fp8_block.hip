@@ -74,6 +74,27 @@ LX2V_DEVICE f32x4 mfma_block(const i32x8& w, const i32x8& a) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);  // (zero scale operands: the form without block scales)
 }
 
+// GELU of N values: x * sigmoid(2u), u = sqrt(2/pi) (x + 0.044715 x^3), as x / (1 + 2^(x (c1 + c3 x^2))).  In stages over all N: a
+// lone wave would wait behind every exp2 and reciprocal of its own (72 cycles a value one after the other, 56 staged; a tile of
+// 192 x 256 holds 192 values a lane).
+template <int N>
+LX2V_DEVICE void gelu(float (&v)[N]) {
+#pragma clang fp reassociate(off)
+  constexpr float C1 = -2.f * 0.7978845608028654f * 1.4426950408889634f, C3 = C1 * 0.044715f;
+  float e[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) e[j] = v[j] * __builtin_fmaf(v[j] * v[j], C3, C1);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < N; ++j) e[j] = __builtin_amdgcn_exp2f(e[j]);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < N; ++j) e[j] = __builtin_amdgcn_rcpf(1.0f + e[j]);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] *= e[j];
+}
+
 // Four consecutive columns n .. n + 3 of row m: bias, then GELU / gated residual, one rounding.
 template <int EPI>
 LX2V_DEVICE void finish4(const Params& p, const f32x4& acc, int64_t m, int n) {
@@ -85,10 +106,7 @@ LX2V_DEVICE void finish4(const Params& p, const f32x4& acc, int64_t m, int n) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] += b[j];
   }
-  if constexpr (EPI == LX2V_EPI_GELU_TANH) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = gelu_tanh(v[j]);
-  }
+  if constexpr (EPI == LX2V_EPI_GELU_TANH) gelu(v);
   if constexpr (EPI == LX2V_EPI_RESIDUAL) {
     if (p.gate != nullptr) {
       const f32x4 g = *reinterpret_cast<const f32x4*>(p.gate + n);
@@ -531,15 +549,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     static_for<0, U>([&](auto uc) __attribute__((always_inline)) {
       constexpr int u = decltype(uc)::value, i = u % MT, k2 = u / MT, b = k2 % CV;
       if constexpr (EPI != LX2V_EPI_RESIDUAL && i == 0 && k2 < NT / 2 - 1) fetch_cols(IntC<k2 + 1>{});
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = acc[i][2 * k2 + (e >> 2)][e & 3] + bv[b][e >> 2][e & 3];
+      if constexpr (EPI == LX2V_EPI_GELU_TANH) gelu(x);
       uint32_t d[2][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = acc[i][2 * k2 + h][e] + bv[b][h][e];
-          if constexpr (EPI == LX2V_EPI_GELU_TANH) v[e] = gelu_tanh(v[e]);
-        }
+        float* v = x + 4 * h;
         if constexpr (EPI == LX2V_EPI_RESIDUAL) {
           const u32x2 r = rv[u % RV][h];
           v[0] = v[0] * gv[b][h][0] + __uint_as_float(r[0] << 16);
@@ -552,9 +569,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       }
       // lane rows fq = 0 .. 3 of block k: columns 4 fq ..; swapping the odd rows of d[0] with the even rows of d[1] leaves row 0
       // with columns 0-7 of block k, row 1 with 0-7 of block k + 1, row 2 with 8-15 of block k, row 3 with 8-15 of block k + 1
-      const auto x = __builtin_amdgcn_permlane16_swap(d[0][0], d[1][0], false, false);
-      const auto y = __builtin_amdgcn_permlane16_swap(d[0][1], d[1][1], false, false);
-      const u32x4 out = {x[0], y[0], x[1], y[1]};
+      const auto lo = __builtin_amdgcn_permlane16_swap(d[0][0], d[1][0], false, false);
+      const auto hi = __builtin_amdgcn_permlane16_swap(d[0][1], d[1][1], false, false);
+      const u32x4 out = {lo[0], hi[0], lo[1], hi[1]};
       if constexpr (EPI != LX2V_EPI_RESIDUAL) {
         store(uc, out);
       } else {
