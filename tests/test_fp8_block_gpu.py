@@ -460,3 +460,18 @@ def test_hunyuan_double_block_with_block_scaled_linears(cuda):
         for got, key, x0 in ((img, "img_out", c["img"]), (txt, "txt_out", c["txt"])):
             ref = torch.from_numpy(rec[key])
             assert cos(got[0], ref) >= 0.999 and cos(got[0].float().cpu() - x0[0], ref - x0[0]) >= 0.99, (name, key)
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 64, 256), (300, 264, 272), (40, 512, 2048)])   # skinny, tile, split along K
+def test_gelu_of_huge_and_infinite_values(cuda, M, N, K):
+    zero = torch.zeros(M, K, device=cuda).to(torch.float8_e4m3fn)
+    a_s = torch.ones((K + 127) // 128, M, device=cuda).t()
+    w = torch.zeros(N, K, device=cuda).to(torch.float8_e4m3fn)
+    w_s = torch.ones((N + 127) // 128, (K + 127) // 128, device=cuda)
+    bias = torch.zeros(N, device=cuda)
+    bias[:8] = torch.tensor([-1e30, 1e30, -25.0, 25.0, 0.0, float("inf"), float("nan"), -3e-39])
+    out = hip.gemm_fp8_block(zero, a_s, w, w_s, bias, epilogue=hip.EPI_GELU_TANH).float()
+    big = torch.tensor(1e30).to(torch.bfloat16).float().item()
+    for col, want in enumerate((0.0, big, 0.0, 25.0, 0.0, float("inf"))):
+        assert bool((out[:, col] == want).all()), (col, out[0, col])
+    assert bool(out[:, 6].isnan().all()) and bool((out[:, 7].abs() <= 3e-39).all()) and bool((out[:, 8:] == 0).all())
