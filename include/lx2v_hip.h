@@ -455,7 +455,10 @@ int lx2v_gemm_fp8_block128(const uint8_t* A, int64_t lda, const float* a_scale, 
  *   LX2V_QUANT_FP8_ROW      e4m3, scale[r], the rule of lx2v_quant_fp8_rowwise      (operand of lx2v_gemm_fp8)
  *   LX2V_QUANT_FP8_GROUP128 e4m3, scale[g * ld_scale + r] per 128 columns           (operand of lx2v_gemm_fp8_block128)
  *   LX2V_QUANT_INT8_ROW     int8, scale[r], the rule of lx2v_quant_int8_rowwise (weight_mode 0)  (operand of lx2v_gemm_int8)
- * (ld_scale is read for GROUP128 only).  Replaces, where a norm feeds a quantised Linear, RMSWeightSgl.apply and the
+ * (ld_scale is read for GROUP128 only).  NaN in x + y makes its whole row NaN; an infinity becomes NaN and the rest of its row
+ * zeros (the row is divided by infinity, as in lx2v_rmsnorm_rope_bf16; so is a row whose sum of squares overflows fp32: one
+ * value of 1.8e19 does).  e4m3 rows carry these as NaN codes; int8 holds none, so there a row with a NaN, an infinity or such an
+ * overflow has a scale of NaN, and the Linear behind it returns NaN.  Replaces, where a norm feeds a quantised Linear, RMSWeightSgl.apply and the
  * activation quantisation behind it  lightx2v/common/ops/norm/rms_norm_weight.py:131-146, mm/mm_weight.py:492-505. */
 #define LX2V_QUANT_FP8_ROW 0
 #define LX2V_QUANT_FP8_GROUP128 1

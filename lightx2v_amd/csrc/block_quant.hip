@@ -5,7 +5,8 @@
 //                        row, or as e4m3 rows with one scale per 128 columns
 // A scale is max(max|group|, 1e-12) / 448 and an element e4m3(v * (1 / scale)), the rule of the row-wise quantiser in
 // step_ew.hip (a row of 128 columns gets the same bytes and scale from both).  The maximum skips NaN (fmaxf) and the NaN
-// element becomes the NaN code; an infinite element makes its group's scale infinite and its own code NaN.  This file
+// element becomes the NaN code; an infinite element makes its group's scale infinite and its own code NaN.  int8 rows have a
+// NaN scale instead.  This file
 // is built with IEEE division and without contraction, so scales and reciprocals are the correctly rounded quotients.
 //
 // Scales per 128 columns are stored group after group (element (r, g) at scale[g * ld_scale + r]): the GEMM reads the
@@ -62,6 +63,13 @@ LX2V_DEVICE float absmax8(const float (&f)[8]) {
 #pragma unroll
   for (int i = 1; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
   return m;
+}
+// The same where nothing may hide a NaN: infinite if any of the eight is infinite or NaN (magnitudes order as their bit patterns do, NaN last).
+LX2V_DEVICE float absmax8_or_inf(const float (&f)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+  return __uint_as_float(min(m, 0x7f800000u));
 }
 LX2V_DEVICE float scale_e4m3(float amax) { return __fdiv_rn(fmaxf(amax, AMAX_FLOOR), E4M3_MAX); }
 LX2V_DEVICE u32x2 cvt8_e4m3(const float (&f)[8], float inv) {
@@ -237,7 +245,8 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(T* x, int64_t ldx, con
         for (int j = 0; j < 8; ++j) f[c][j] *= g[j];
       }
       if constexpr (FORM == FORM_BF16) store8<BIG>(static_cast<uint16_t*>(out) + row * ldo + ch * 8, f[c]);
-      if constexpr (FORM == FORM_ROW || FORM == FORM_INT8) amax = fmaxf(amax, absmax8(f[c]));
+      if constexpr (FORM == FORM_ROW) amax = fmaxf(amax, absmax8(f[c]));
+      if constexpr (FORM == FORM_INT8) amax = fmaxf(amax, absmax8_or_inf(f[c]));
     }
     if constexpr (FORM == FORM_GROUP) {  // (outside the branch: lanes past the row's end hold zeros and take part in the rotations)
       const float sc = scale_e4m3(max16(absmax8(f[c])));
@@ -254,7 +263,9 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(T* x, int64_t ldx, con
       __syncthreads();
       amax = fmaxf(fmaxf(part[1][0], part[1][1]), fmaxf(part[1][2], part[1][3]));
     }
-    const float sc = FORM == FORM_ROW ? scale_e4m3(amax) : __fdiv_rn(amax, 127.0f);
+    // int8 codes hold no NaN, so a row with one (in its elements, or because its sum of squares is not finite) says so in its scale
+    const bool lost = FORM == FORM_INT8 && !(ss < INFINITY && amax < INFINITY);
+    const float sc = FORM == FORM_ROW ? scale_e4m3(amax) : lost ? NAN : __fdiv_rn(amax, 127.0f);
     const float inv = FORM == FORM_ROW ? __frcp_rn(sc) : amax > 0.f ? __fdiv_rn(127.0f, amax) : 0.f;
     if (t == 0) scale[row] = sc;
 #pragma unroll
