@@ -374,7 +374,9 @@ int lx2v_gemm_fp8(const uint8_t* A, int64_t lda, const float* a_scale, const uin
  *   symmetric=True), dynamic per-token)  lightx2v/common/ops/mm/mm_weight.py:503-505.
  * weight_mode 1, weights per output channel: scale[r] = max(max|x[r,:]|, 1e-5) / 127 ; out = rint(x / scale[r]).
  *   Replaces IntegerQuantizer(8, True, "per_channel").real_quant_tensor as load_int8_perchannel_sym uses it
- *   lightx2v/common/ops/mm/mm_weight.py:322-330, lightx2v/utils/quant_utils.py:39-49,85-92,111-113. */
+ *   lightx2v/common/ops/mm/mm_weight.py:322-330, lightx2v/utils/quant_utils.py:39-49,85-92,111-113.
+ * NaN does not count in the maximum and becomes the code -128 (a row of nothing else: scale 0, in weight_mode 1 1e-5 / 127); an
+ * infinite element makes the scale infinite and its own code -128.  Nothing of either is marked: int8 codes hold no NaN. */
 int lx2v_quant_int8_rowwise(const uint16_t* x, int64_t ldx, int8_t* out, int64_t ldo, float* scale,
                             int64_t rows, int dim, int weight_mode, void* stream);
 /* From fp32 rows (mm_weight.py:324-327 quantises `weight.to(torch.float32)`). */
