@@ -59,7 +59,9 @@ LX2V_DEVICE void static_for(F&& f) {
   }
 }
 
-// (an operand tile of at most 256 rows, each below 8 MiB: the extent is below 2^31 and computed in 32 bits)
+// Raw buffer of `bytes` from `base`: an access is out of range, and loads 0, when its vector and scalar offsets together reach the extent
+// (measured for plain loads and LDS-DMA: neither a scalar offset past the extent nor an extent of 0 makes the comparison wrap).
+// An operand tile has at most 256 rows, each below 4 MiB: its extent is below 2^31 and computed in 32 bits.
 LX2V_DEVICE u32x4 raw_descriptor(const void* base, uint32_t bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(base);
   u32x4 d;
@@ -243,7 +245,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   };
   struct Cursor {
     int ord = 0, kt = 0;
-    uint32_t soff = 0;
+    uint32_t soff = 0, step = BK;  // (past the last tile no step: with an empty descriptor a load's scalar offset stays 0 too)
   } ca, cw;
   u32x4 a_rs, w_rs;
   uint64_t s_base = 0, s_step = 0;  // the scales' descriptor: its base moves on by a block's scales, its extent stays
@@ -260,7 +262,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     tile_origin(raster, vbid, T::TM, T::TN, m0, n0);
     const int rows = vbid < ntiles ? min(M - m0, T::TM) : 0;
     a_rs = raw_descriptor(reinterpret_cast<const uint8_t*>(base) + (int64_t)(rows ? m0 : 0) * lda, (uint32_t)rows * (uint32_t)lda);
-    asm volatile("" : "+s"(a_rs));
+    ca.step = rows ? BK : 0;
+    asm volatile("" : "+s"(a_rs), "+s"(ca.step));
   };
   auto w_tile = [&]() __attribute__((always_inline)) {
     const ParamsAgain p = params_again();
@@ -277,9 +280,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     w_rs = raw_descriptor(reinterpret_cast<const uint8_t*>(base) + (int64_t)n0 * ldw, (uint32_t)rows * (uint32_t)ldw);
     const int nb = min(((N + 127) >> 7) - (n0 >> 7), (T::TN + 127) / 128);  // weight row blocks of the tile
     const float* sb = sw_wave ? reinterpret_cast<const float*>(wsb) + (int64_t)(n0 >> 7) * lds_w + kb0 : reinterpret_cast<const float*>(asb) + (int64_t)kb0 * lds_a + m0;
+    cw.step = live ? BK : 0;
     s_base = reinterpret_cast<uint64_t>(sb);
     s_bytes = !live ? 0u : sw_wave ? ((uint32_t)(nb - 1) * (uint32_t)lds_w + 1) * 4 : (uint32_t)min(M - m0, T::TM) * 4;
-    asm volatile("" : "+s"(w_rs), "+s"(s_base), "+s"(s_bytes));
+    asm volatile("" : "+s"(w_rs), "+s"(s_base), "+s"(s_bytes), "+s"(cw.step));
     s_pv = sw_wave ? (lane < nb ? lane * (int)lds_w * 4 : NOWHERE) : (64 * wid + lane) * 4;
   };
   a_tile();
@@ -339,7 +343,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     constexpr int i = decltype(ic)::value;
     if constexpr (i == 0) {
       ++cw.kt;
-      cw.soff += BK;
+      cw.soff += cw.step;
       s_base += s_step;
       asm volatile("" : "+s"(cw.kt), "+s"(cw.soff), "+s"(s_base));
     } else if constexpr (i == 1 && !TWO) {
@@ -352,7 +356,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       asm volatile("" : "+s"(s_cur), "+s"(s_nxt));
     } else if constexpr (i == 3) {
       ++ca.kt;
-      ca.soff += BK;
+      ca.soff += ca.step;
       a_cur = a_nxt;
       a_nxt = a_nxt == dma_base + (T::SA - 1) * T::A_BYTES ? dma_base : a_nxt + T::A_BYTES;
       asm volatile("" : "+s"(ca.kt), "+s"(ca.soff), "+s"(a_cur), "+s"(a_nxt));
@@ -367,7 +371,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       w_tile();
       if (ragged >= 0) w_pv = offset(params_again()->ldw, ragged == 0);
     }
-    asm volatile("" : "+s"(w_rs), "+s"(s_base), "+s"(s_bytes), "+s"(cw.soff), "+s"(cw.kt), "+s"(cw.ord), "+s"(dma_base), "+s"(dma_sc));
+    asm volatile("" : "+s"(w_rs), "+s"(s_base), "+s"(s_bytes), "+s"(cw.soff), "+s"(cw.step), "+s"(cw.kt), "+s"(cw.ord), "+s"(dma_base), "+s"(dma_sc));
   };
   auto a_turn = [&]() __attribute__((always_inline)) {
     if (ca.kt == ragged) a_pv = offset(params_again()->lda, true);
@@ -378,7 +382,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       a_tile();
       if (ragged >= 0) a_pv = offset(params_again()->lda, ragged == 0);
     }
-    asm volatile("" : "+s"(a_rs), "+s"(ca.soff), "+s"(ca.kt), "+s"(ca.ord), "+s"(a_cur), "+s"(a_nxt));
+    asm volatile("" : "+s"(a_rs), "+s"(ca.soff), "+s"(ca.step), "+s"(ca.kt), "+s"(ca.ord), "+s"(a_cur), "+s"(a_nxt));
   };
 
   // ---- fragments: register set P (0 | 1) = NT W fragments, then MT A fragments, of 8 accumulator registers each ----

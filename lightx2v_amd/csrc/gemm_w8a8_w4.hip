@@ -118,6 +118,9 @@ LX2V_DEVICE void acc_to_global(int voff, const f32x4& acc, uint64_t sbase) {
   else asm volatile("global_store_dwordx4 %0, %1, %2" ::"v"(voff), "v"(acc), "s"(sbase) : "memory");
 }
 
+// Raw buffer of `bytes` from `base`: an access is out of range, and loads 0, when its vector offset (offset field included) and scalar
+// offset together reach the extent (measured for plain loads and LDS-DMA: neither a scalar offset past the extent nor an extent of 0, as the
+// stream's last two K-tiles have, makes the comparison wrap).
 LX2V_DEVICE u32x4 raw_descriptor(const void* base, int64_t bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(base);
   u32x4 d;
