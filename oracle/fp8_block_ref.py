@@ -72,3 +72,26 @@ def add_rmsnorm(x, y, w, eps):
     h = x.double() + (0 if y is None else y.double())
     v = h / torch.sqrt((h * h).mean(dim=1, keepdim=True) + eps)
     return h, v if w is None else v * w.double()
+
+
+def whole_operands(M, N, K, seed, device="cpu"):
+    """(a8, a_scale, w8, w_scale) whose products and sums are whole numbers that the fp8 MFMA and fp32 hold exactly, so that a correct
+    product equals the 64-bit one before its rounding to bf16, whatever the order of its sums.  Dequantised, |a| and |w| are 2, here
+    and there 1 or 3; the second half of K has a negative, so that sums grow to 2 K on the way and come back to the order of sqrt(K):
+    mostly below 256, where bf16 has steps of at most 1 and every single product (1 to 9) shows.  Scales are powers of two that
+    differ from block to block, the codes hold their inverse."""
+    g = torch.Generator(device=device).manual_seed(seed)
+
+    def near_two(rows):
+        r = torch.randint(0, 16, (rows, K), generator=g, device=device)
+        return 2.0 + (r == 0).float() - (r == 1).float()
+
+    def powers(rows):
+        return torch.exp2(torch.randint(-3, 4, (rows, (K + BLOCK - 1) // BLOCK), generator=g, device=device).float())
+
+    a, w = near_two(M), near_two(N)
+    a[:, K // 2:] *= -1
+    a_scale, w_scale = powers(M), powers((N + BLOCK - 1) // BLOCK)
+    a = a / a_scale.repeat_interleave(BLOCK, dim=1)[:, :K]
+    w = w / w_scale.repeat_interleave(BLOCK, dim=0)[:N].repeat_interleave(BLOCK, dim=1)[:, :K]
+    return a.to(torch.float8_e4m3fn), a_scale.t().contiguous().t(), w.to(torch.float8_e4m3fn), w_scale
