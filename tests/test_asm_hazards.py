@@ -66,6 +66,28 @@ def test_checker_flags_an_lds_read_destination_touched_before_a_wait(tmp_path):
     assert _run(tmp_path, between=read + "\tv_mov_b32_e32 v20, v21") == 0                   # other registers
 
 
+def test_checker_counts_the_wait_states_behind_an_mfma(tmp_path):
+    """20 wait states of the author's own, one after the other, are longer than any MFMA takes: what follows may touch its destination."""
+    read, plain = "\tv_mul_f32_e32 v3, v14, v36", "\tv_mov_b32_e32 v20, v21\n"
+
+    def nops(*counts, asm=True):
+        t = "".join(f"\ts_nop {c}\n" for c in counts)
+        return f"\t;;#ASMSTART\n{t}\t;;#ASMEND\n" if asm else t
+
+    assert _run(tmp_path, between=nops(7, 7, 7) + read) == 0                                  # 24
+    assert _run(tmp_path, between=nops(7, 7, 3) + read) == 0                                  # 20
+    assert _run(tmp_path, between=nops(7, 7, 2) + read) == 1                                  # 19
+    assert _run(tmp_path, between=nops(7, 7) + read) == 1                                     # 16
+    assert _run(tmp_path, between=nops(7, 7) + nops(7) + read) == 0                           # in two asm statements, one behind the other
+    assert _run(tmp_path, between=nops(7, 7, 7, asm=False) + read) == 1                       # the compiler's own, which serve its own hazards
+    assert _run(tmp_path, between=nops(7, 7) + nops(7, asm=False) + read) == 1
+    assert _run(tmp_path, between=nops(7) + plain + nops(7, 7) + read) == 1                   # an instruction in between
+    assert _run(tmp_path, between=nops(7) + read + "\n" + nops(7, 7)) == 1                    # too late
+    assert _run(tmp_path, between=nops(7, 7) + ".LBB0_2:\n" + nops(7) + read) == 1            # a jump may land behind the first two
+    mfma = "\t;;#ASMSTART\n\tv_mfma_f32_16x16x32_bf16 v[12:15], v[74:77], a[44:47], v[12:15]\n\t;;#ASMEND\n"
+    assert _run(tmp_path, between=nops(7, 7, 7) + mfma + read) == 1                           # the next MFMA's destination is its own matter
+
+
 @pytest.mark.skipif(shutil.which("hipcc") is None, reason="needs hipcc")
 def test_kernels_with_inline_asm_mfmas_are_clean():
     r = subprocess.run(["make", "-C", os.path.join(ROOT, "lightx2v_amd", "csrc"), "-j4", "asmcheck"], capture_output=True, text=True, timeout=1500)

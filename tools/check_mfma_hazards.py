@@ -7,7 +7,7 @@ then do silently break results:
   * touch the VGPR destination of an inline-asm MFMA (a copy when it splits a live range, say) before
     the MFMA has written it -- an error when a compiler-generated instruction reads or writes such
     registers before any further MFMA has been issued (the next MFMA issues when the pipe is free,
-    which is when the first one has finished its passes) and before 20 wait states of inline-asm s_nop,
+    which is when the first one has finished its passes) and before 20 wait states of inline-asm s_nop in a row,
     counted as a note when one MFMA lies between.  MFMAs the compiler emitted itself (builtins) are its own business: it knows their latency;
   * move data through the ring registers -- flagged for any compiler-generated instruction that
     names a register at or above --ring-base;
@@ -50,15 +50,18 @@ def check(path, kernel_filter, ring_base):
             if t.startswith(";;#ASMEND"):
                 in_asm = False
                 continue
-            if not t or t.startswith(";") or t.startswith(".") or t.endswith(":"):
-                continue
-            rows.append((t.split(";")[0].strip(), in_asm))
+            t = t.split(";")[0].strip()
+            if t.endswith(":"):
+                rows.append(("label", False))  # a jump may land here: wait states in front of it do not count behind it
+            elif t and not t.startswith("."):
+                rows.append((t, in_asm))
         pending = []  # [regs, mfmas_seen, text]
         landing = []  # [regs, text] of asm LDS reads into VGPRs that no wait has covered yet
         notes = 0
         nops = 0
         for t, from_asm in rows:
-            # wait states the author wrote behind the last MFMA: 20 are more than any of these instructions takes to write its result
+            # wait states the author wrote behind the last MFMA, one after the other: 20 are what the longest of these instructions (16 passes)
+            # takes to write its result
             nops = nops + int(t.split()[1]) + 1 if from_asm and t.startswith("s_nop") else 0
             if nops >= 20:
                 pending = []
