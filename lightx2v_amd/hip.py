@@ -99,6 +99,12 @@ def load() -> ctypes.CDLL:
             "lightx2v_amd has no CPU or PyTorch fallback for its ops."
         )
     lib = ctypes.CDLL(path)
+    rebuild = "rebuild it with `make -C lightx2v_amd/csrc` (or __graft_entry__.build())"
+    missing = [name for name in EXPORTS if not hasattr(lib, name)]   # (entry points are added without a new version number)
+    if missing:
+        raise RuntimeError(f"{path} lacks {len(missing)} of this package's entry points ({', '.join(missing[:3])}{', ...' if len(missing) > 3 else ''}): it was built from other sources, {rebuild}")
+    if lib.lx2v_abi_version() != ABI_VERSION:
+        raise RuntimeError(f"{path} has ABI version {lib.lx2v_abi_version()}, this package needs {ABI_VERSION}: {rebuild}")
     for name, argtypes in _SIGNATURES.items():
         fn = getattr(lib, name)
         fn.argtypes = argtypes

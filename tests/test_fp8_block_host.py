@@ -1,5 +1,7 @@
 """Refusals of the block-scaled e4m3 Linear, its quantisers and the residual RMSNorm: nothing is launched, no GPU is needed."""
 import ctypes
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -116,3 +118,27 @@ def test_plugin_is_registered_and_refuses_what_does_not_fit():
             cls("w.weight", None).load({"w.weight": torch.zeros(128, 128)})
     assert [L.MM_WEIGHT_REGISTER[n].norm_form for n in ("hip-bf16", "hip-fp8", "hip-int8", "hip-fp8-block128")] == [None, "row", "int8", "group"]
     assert "hip-fp8-block128" in L.WanTransformerWeights({"num_layers": 1, "num_heads": 2, "dim": 256, "task": "t2v", "dit_quant_scheme": "hip-fp8-block128"}).mm_type
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="needs gcc")
+def test_a_library_of_other_sources_is_refused_by_name(tmp_path, monkeypatch):
+    def built(name, skip, version):
+        src = tmp_path / f"{name}.c"
+        src.write_text("".join(f"int {e}(void) {{ return {version if e == 'lx2v_abi_version' else 0}; }}\n" for e in hip.EXPORTS if e not in skip))
+        so = tmp_path / f"{name}.so"
+        subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(so), str(src)], check=True)
+        return str(so)
+
+    monkeypatch.setattr(hip, "_lib", None)
+    older = built("older", ("lx2v_gemm_fp8_block128", "lx2v_quant_fp8_group128"), hip.ABI_VERSION)
+    monkeypatch.setattr(hip, "lib_path", lambda: older)
+    with pytest.raises(RuntimeError, match="lacks 2 of .*lx2v_quant_fp8_group128, lx2v_gemm_fp8_block128.* rebuild"):
+        hip.load()
+    other = built("other", (), hip.ABI_VERSION + 1)
+    monkeypatch.setattr(hip, "lib_path", lambda: other)
+    with pytest.raises(RuntimeError, match=f"ABI version {hip.ABI_VERSION + 1}, .* needs {hip.ABI_VERSION}"):
+        hip.load()
+    assert hip._lib is None
+    same = built("same", (), hip.ABI_VERSION)
+    monkeypatch.setattr(hip, "lib_path", lambda: same)
+    assert hip.load() is hip._lib is not None
