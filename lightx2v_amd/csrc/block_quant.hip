@@ -23,6 +23,7 @@ constexpr float AMAX_FLOOR = 1e-12f;
 // [75600, 5120] to e4m3 groups 463 against 514.  Below, the producer's result is still there and the consumer finds this
 // one's: norm of [32760, 1536] to e4m3 rows 53 us against 66 with them.
 constexpr int64_t STREAMED_BYTES = 512 << 20;
+constexpr int MAX_DIM = 0x7fffffff - 511;  // columns are counted in 32 bits, in steps of at most 512
 constexpr int64_t MAX_BLOCKS = 1 << 24;  // of 256 threads: a dimension of a launch has less than 2^32 threads
 
 template <bool BIG, class V>
@@ -334,6 +335,7 @@ template <class T>
 int quant_group128(const T* x, int64_t ldx, const lx2v_kseg* kseg, uint8_t* out, int64_t ldo, float* scale, int64_t lds, int64_t rows, int dim, void* stream) {
   LX2V_REQUIRE(rows == 0 || (x && out && scale), LX2V_EINVAL, "quant_fp8_group128: null tensor");
   LX2V_REQUIRE(rows >= 0 && dim > 0 && dim % 8 == 0, LX2V_EINVAL, "quant_fp8_group128: dim=%d must be a positive multiple of 8", dim);
+  LX2V_REQUIRE(dim <= MAX_DIM, LX2V_EUNSUP, "quant_fp8_group128: dim=%d, at most %d columns are supported", dim, MAX_DIM);
   LX2V_REQUIRE(ldx % 8 == 0 && ldo % 8 == 0 && ldo >= dim, LX2V_EINVAL, "quant_fp8_group128: row strides must be multiples of 8, the output's >= dim");
   LX2V_REQUIRE(lx2v_aligned16(x) && (reinterpret_cast<uintptr_t>(out) & 7u) == 0, LX2V_EINVAL, "quant_fp8_group128: x must be 16-byte, out 8-byte aligned");
   LX2V_REQUIRE(lds >= rows, LX2V_EINVAL, "quant_fp8_group128: the stride between groups of scales must be >= rows");
@@ -354,11 +356,11 @@ template <class T>
 int quant_block128(const T* x, int64_t ldx, uint8_t* out, int64_t ldo, float* scale, int64_t lds, int64_t rows, int dim, void* stream) {
   LX2V_REQUIRE(rows == 0 || (x && out && scale), LX2V_EINVAL, "quant_fp8_block128: null tensor");
   LX2V_REQUIRE(rows >= 0 && dim > 0 && dim % 8 == 0, LX2V_EINVAL, "quant_fp8_block128: dim=%d must be a positive multiple of 8", dim);
+  LX2V_REQUIRE(dim <= MAX_DIM, LX2V_EUNSUP, "quant_fp8_block128: dim=%d, at most %d columns are supported", dim, MAX_DIM);
   LX2V_REQUIRE(ldx % 8 == 0 && ldo % 8 == 0 && ldx >= dim && ldo >= dim, LX2V_EINVAL, "quant_fp8_block128: row strides must be multiples of 8 and >= dim");
   LX2V_REQUIRE(lx2v_aligned16(x) && (reinterpret_cast<uintptr_t>(out) & 7u) == 0, LX2V_EINVAL, "quant_fp8_block128: x must be 16-byte, out 8-byte aligned");
   LX2V_REQUIRE(lds >= (dim + 127) / 128, LX2V_EINVAL, "quant_fp8_block128: the row stride of the scales must be >= ceil(dim / 128)");
   LX2V_REQUIRE((rows + 127) / 128 <= 65535, LX2V_EUNSUP, "quant_fp8_block128: rows=%lld, at most 65535 blocks of 128 are supported", (long long)rows);
-  LX2V_REQUIRE((dim + 127) / 128 < MAX_BLOCKS, LX2V_EUNSUP, "quant_fp8_block128: dim=%d is too large", dim);
   if (rows == 0) return LX2V_OK;
   hipLaunchKernelGGL(quant_fp8_block128_kernel<T>, dim3((unsigned)((dim + 127) / 128), (unsigned)((rows + 127) / 128)), dim3(256), 0, (hipStream_t)stream, x, ldx, out, ldo, scale, lds,
                      rows, dim);

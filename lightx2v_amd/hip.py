@@ -776,6 +776,7 @@ def gemm_fp8(a8: torch.Tensor, a_scale: torch.Tensor, w8: torch.Tensor, w_scale:
 
 # ------------------------------------------------------------------------------- block-scaled fp8
 BLOCK = 128  # columns of K (and rows of a weight) that share one scale
+_MAX_DIM = 2 ** 31 - 512  # the entry points count columns in 32 bits
 
 
 class QuantGroups(QuantRows):
@@ -798,6 +799,8 @@ def _need_float_rows(name: str, t: torch.Tensor) -> bool:
     """bf16 or fp32 GPU [rows, dim] with a contiguous innermost dimension; True for fp32."""
     if t.dim() != 2:
         raise Lx2vError(f"{name}: expected [rows, dim], got shape {tuple(t.shape)}")
+    if t.shape[1] > _MAX_DIM:
+        raise Lx2vError(f"{name}: {t.shape[1]} columns, at most {_MAX_DIM} are supported")
     if t.dtype is torch.float32:
         if not t.is_cuda or (t.stride(1) != 1 and t.shape[1] > 1):
             raise Lx2vError(f"{name}: fp32 input must be a GPU matrix with a contiguous inner dimension")
@@ -837,6 +840,8 @@ def quant_fp8_group128(x: torch.Tensor, kseg: Optional["KSeg"] = None, dim: Opti
         raise Lx2vError("quant_fp8_group128: a segmented source is bf16 and needs `dim`")
     rows, width = x.shape
     dim = width if kseg is None else int(dim)
+    if dim > _MAX_DIM:
+        raise Lx2vError(f"quant_fp8_group128: {dim} columns, at most {_MAX_DIM} are supported")
     device = x.device
     q = torch.empty((rows, dim), dtype=torch.float8_e4m3fn, device=device)
     scale = _group_scales(rows, dim, device)

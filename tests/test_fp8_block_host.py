@@ -142,3 +142,16 @@ def test_a_library_of_other_sources_is_refused_by_name(tmp_path, monkeypatch):
     same = built("same", (), hip.ABI_VERSION)
     monkeypatch.setattr(hip, "lib_path", lambda: same)
     assert hip.load() is hip._lib is not None
+
+
+def test_more_columns_than_32_bits_count_are_refused(p):
+    """2^32 + 8 columns would reach the entry points as 8."""
+    lib, big, ld = hip.load(), 2 ** 31 - 8, 1 << 31
+    assert lib.lx2v_quant_fp8_group128(p, ld, None, p, ld, p, 1, 1, big, None) == -2 and b"columns" in lib.lx2v_last_error()
+    assert lib.lx2v_quant_fp8_group128_f32(p, ld, p, ld, p, 1, 1, big, None) == -2 and b"columns" in lib.lx2v_last_error()
+    assert lib.lx2v_quant_fp8_block128(p, ld, p, ld, p, ld, 1, big, None) == -2 and b"columns" in lib.lx2v_last_error()
+    assert lib.lx2v_quant_fp8_block128_f32(p, ld, p, ld, p, ld, 1, big, None) == -2 and b"columns" in lib.lx2v_last_error()
+    wide = torch.empty(1, 2 ** 32 + 8, dtype=torch.bfloat16, device="meta")
+    for call in (lambda: hip.quant_fp8_group128(wide), lambda: hip.quant_fp8_block128(wide), lambda: hip.add_rmsnorm_(wide, None)):
+        with pytest.raises(hip.Lx2vError, match="columns"):
+            call()
