@@ -99,3 +99,23 @@ def test_error_is_that_of_the_rounding_in_every_row(cuda, M, N, K, epi):
     assert float(err.norm() / v.norm()) <= bound
     rows = err.norm(dim=1) / v.norm(dim=1)
     assert bool((rows <= bound).all()), (int(rows.argmax()), float(rows.max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(300, 520, 13840), (512, 2560, 16400), (262, 4096, 13840), (2179, 1032, 13840), (900, 1288, 96), (13, 520, 272)])
+def test_largest_row_strides(cuda, M, N, K):
+    """Rows as far apart as the entry point takes them: the offsets inside a tile come near 2^30 (operands) and 2^31 bytes (results)."""
+    (aq, a_s, wq, w_s), a, w = _whole(M, N, K, 7, cuda)
+    far = lambda rows, ld, dtype: torch.empty_strided((rows, ld), (ld, 1), dtype=dtype, device=cuda)
+    wide_a, wide_w = (far(r, (1 << 22) - 16, torch.uint8)[:, -K:] for r in (M, N))
+    wide_a.copy_(aq.view(torch.uint8))
+    wide_w.copy_(wq.view(torch.uint8))
+    out, resid = (far(M, (1 << 22) - 8, torch.bfloat16)[:, -N:] for _ in range(2))
+    resid.fill_(3.0)
+    v = a @ w.t().contiguous()
+    for ws in (None, torch.empty(16, dtype=torch.uint8, device=cuda)):    # split along K where the plan says so, and whole
+        args = (wide_a.view(torch.float8_e4m3fn), a_s, wide_w.view(torch.float8_e4m3fn), w_s)
+        out.fill_(float("nan"))
+        assert torch.equal(hip.gemm_fp8_block(*args, out=out, workspace=ws), v.to(torch.bfloat16))
+        hip.gemm_fp8_block(*args, epilogue=hip.EPI_RESIDUAL, resid=resid, out=out, workspace=ws)
+        assert torch.equal(out, (v + 3).to(torch.bfloat16))

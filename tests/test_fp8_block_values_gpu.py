@@ -46,3 +46,19 @@ def test_int8_row_whose_sum_of_squares_overflows_has_a_nan_scale(cuda, stream):
     x[1, 5], x[2] = 1e30, 3e38
     r = hip.add_rmsnorm_(x.clone(), None, None, quant="int8")
     assert bool(r.scale[1:3].isnan().all()) and bool(r.scale[[0, 3]].isfinite().all()) and bool((r.q[[0, 3]] == 127).all())
+
+
+@pytest.mark.parametrize("seg,seg2", [(64, 8), (8, 256), (128, 128), (200, 40)])
+def test_quant_of_a_source_in_two_regions(cuda, seg, seg2):
+    """Column segments of two widths (a sequence-parallel result with its own remainder): groups of 128 columns astride them."""
+    rows, n, n2 = 37, 4, 3
+    g = torch.Generator(device=cuda).manual_seed(6)
+    flat = torch.randn(rows * (n * seg + n2 * seg2) + 16, generator=g, device=cuda).to(torch.bfloat16)
+    base2 = rows * n * seg
+    first = flat[:base2].view(n, rows, seg)
+    second = flat[base2:base2 + rows * n2 * seg2].view(n2, rows, seg2)
+    plain = torch.cat([first.permute(1, 0, 2).reshape(rows, -1), second.permute(1, 0, 2).reshape(rows, -1)], dim=1).contiguous()
+    ks = hip.KSeg(seg=seg, stride=rows * seg, split=n * seg, seg2=seg2, stride2=rows * seg2, base2=base2, lda2=seg2)
+    q, s = hip.quant_fp8_group128(first[0], kseg=ks, dim=plain.shape[1])
+    want_q, want_s = hip.quant_fp8_group128(plain)
+    assert torch.equal(q.view(torch.uint8), want_q.view(torch.uint8)) and torch.equal(s, want_s)
