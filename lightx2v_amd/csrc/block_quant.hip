@@ -19,8 +19,8 @@ constexpr float E4M3_MAX = 448.0f;
 constexpr float AMAX_FLOOR = 1e-12f;
 
 // Non-temporal accesses (BIG) for calls whose tensors are together more than twice the 256 MB memory-side cache, so that
-// nothing of them would be found there again: group quantiser at [75600, 13824] 505 us against 617 without, norm of
-// [75600, 5120] to e4m3 groups 463 against 514.  Below, the producer's result is still there and the consumer finds this
+// nothing of them would be found there again: group quantiser at [75600, 13824] 535 us against 641 without, norm of
+// [75600, 5120] to e4m3 groups 466 against 511 (kernels on a card that ran 501 and 461 at other times).  Below, the producer's result is still there and the consumer finds this
 // one's: norm of [32760, 1536] to e4m3 rows 53 us against 66 with them.
 constexpr int64_t STREAMED_BYTES = 512 << 20;
 constexpr int MAX_DIM = 0x7fffffff - 511;  // columns are counted in 32 bits, in steps of at most 512
@@ -103,9 +103,9 @@ __global__ __launch_bounds__(256) void quant_fp8_group128_kernel(const T* x, int
   for (int i = 0; i < QR; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[i][j] = 0.f;
-  // Short calls load rows past the last one again, so that no branch parts the loads ([257, 1280] 3.6 us against 4.5, [4680, 5120]
-  // 13.7 against 15.3).  Long ones wait for each row's before the next row's test: fewer loads at a time, alike at most sizes
-  // and better at the largest ([75600, 13824] 504 us against 527, [75600, 5120] 195 against 187, [37800, 13824] 260 both).
+  // Short calls load rows past the last one again, so that no branch parts the loads ([257, 1280] 4.5 us of kernel against
+  // 5.3, [4680, 5120] 16.5 against 18.2, inputs from memory).  Long ones wait for each row's before the next row's test: fewer loads
+  // at a time, alike at most sizes and better at the largest ([75600, 13824] 535 us against 553, [75600, 5120] 204 against 200).
   if constexpr (BIG) {
 #pragma unroll
     for (int i = 0; i < QR; ++i)
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(T* x, int64_t ldx, con
   float f[NC][8];
   float ss = 0.f;
   // As in the group quantiser: short calls load without branches in between (lanes past the row's end its last chunk again; one row
-  // of 5120 3.3 us against 3.7, [4680, 5120] 32.2 against 34.0), long ones chunk by chunk ([75600, 5120] 481 against 491).
+  // of 5120 3.4 us of kernel against 3.9, [4680, 5120] 36.4 against 39.3), long ones chunk by chunk ([75600, 5120] 466 against 478).
   if constexpr (BIG) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {

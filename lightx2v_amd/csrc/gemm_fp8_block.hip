@@ -759,14 +759,16 @@ struct Plan {
 // Up to 32 rows the skinny kernel (13 x 5120 x 4096: 9.4 us, the 64 x 128 tile split four ways 12.6; 32 x 5120 x 5120: 12.4 and 14.5;
 // at 64 rows its reads of A cost more than they save, 17.4 and 15.2).  Above, the kernel and split whose estimated time is least.
 // A tile kernel's time is rounds of tiles, each of K blocks and an overhead (pipeline fill, epilogue, tile switch); measured with
-// one tile on nearly every CU, K = 2560 and 10240:
+// one tile on nearly every CU, K = 2560 and 10240 (the estimate of a long run of tiles is too large: 551 us at 32760 x 8960 x 1536 + GELU,
+// which takes 497; the estimates are only compared with each other):
 //   tile        us per K block   us per tile
 //   192 x 256        1.08            10          (one wave's 48 MFMAs are 0.64 us at 2.4 GHz; the CU's LDS moves 168 KB meanwhile)
 //   128 x 256        0.84             8
 //   128 x 128        0.55             5
 //   64 x 128         0.41             3
 // A split along K adds a launch that reads the partial sums back: 5 us and their bytes, written and read, at 4 TB/s.
-// (512 x 10240 x 5120: 128 x 256 whole 35.7 us, 192 x 256 44.9, 128 x 128 47.6; 2500 x 1536 x 8960: 128 x 128 whole 43.1,
+// (Calls in a row on the same operands, weights from the memory-side cache; 512 x 10240 x 5120 takes 46 us with all of them from memory.
+// 512 x 10240 x 5120: 128 x 256 whole 35.7 us, 192 x 256 44.9, 128 x 128 47.6; 2500 x 1536 x 8960: 128 x 128 whole 43.1,
 // 128 x 256 in two parts 46.4; 64 x 5120 x 5120: 64 x 128 in four parts 15.2, whole 20.2; 200 x 5120 x 13824: in three 29.5, 43.9.)
 Plan make_plan(int64_t M, int64_t N, int64_t K, int cus) {
   const int nk = (int)((K + BK - 1) / BK);
