@@ -236,7 +236,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   // piece q of wave w: rows 32 q + 8 w + (lane >> 3) of the operand tile; the swizzle is the same for all q
   const int chunk = (lane & 7) ^ ((4 * wid + (lane >> 4)) & 7);
   const int left = p.K - (p.nk - 1) * BK;  // columns of the last block
-  const int ragged = left < BK && kb0 + nk == p.nk ? nk - 1 : -1;
+  const uint32_t last = (uint32_t)(kb0 + nk - 1) * BK;  // offset in a row of the tile's last block ...
+  const uint32_t ragged = left < BK && kb0 + nk == p.nk ? last : ~0u;  // ... and of its last block if that is short
   int a_pv, w_pv, s_pv = NOWHERE;
   auto offset = [&](int64_t ld, bool last) __attribute__((always_inline)) -> int {  // of piece 0; `last`: chunks past K go nowhere
     int at = (8 * wid + (lane >> 3)) * (int)ld + chunk * 16;
@@ -244,8 +245,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     return last & (chunk * 16 >= left) ? NOWHERE : at;
   };
   struct Cursor {
-    int ord = 0, kt = 0;
-    uint32_t soff = 0, step = BK;  // (past the last tile no step: with an empty descriptor a load's scalar offset stays 0 too)
+    int ord = 0;
+    uint32_t soff = 0, step = BK;  // the block's offset in a row (past the last tile it stays 0: an empty descriptor has no scalar offset either)
   } ca, cw;
   u32x4 a_rs, w_rs;
   uint64_t s_base = 0, s_step = 0;  // the scales' descriptor: its base moves on by a block's scales, its extent stays
@@ -288,8 +289,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   };
   a_tile();
   w_tile();
-  a_pv = offset(p.lda, ragged == 0);
-  w_pv = offset(p.ldw, ragged == 0);
+  a_pv = offset(p.lda, nk == 1 && ragged == last);
+  w_pv = offset(p.ldw, nk == 1 && ragged == last);
   ca.soff = cw.soff = (uint32_t)kb0 * BK;
   {
     const int64_t step = sw_wave ? 4 : p.lds_a * 4;
@@ -342,10 +343,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   auto move = [&](auto ic) __attribute__((always_inline)) {
     constexpr int i = decltype(ic)::value;
     if constexpr (i == 0) {
-      ++cw.kt;
       cw.soff += cw.step;
       s_base += s_step;
-      asm volatile("" : "+s"(cw.kt), "+s"(cw.soff), "+s"(s_base));
+      asm volatile("" : "+s"(cw.soff), "+s"(s_base));
     } else if constexpr (i == 1 && !TWO) {
       w_cur = w_nxt;
       w_nxt = w_nxt == dma_base + (T::SW - 1) * T::W_BYTES ? dma_base : w_nxt + T::W_BYTES;
@@ -355,34 +355,31 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       s_nxt = s_nxt == dma_sc + (T::SW - 1) * 1024 ? dma_sc : s_nxt + 1024;
       asm volatile("" : "+s"(s_cur), "+s"(s_nxt));
     } else if constexpr (i == 3) {
-      ++ca.kt;
       ca.soff += ca.step;
       a_cur = a_nxt;
       a_nxt = a_nxt == dma_base + (T::SA - 1) * T::A_BYTES ? dma_base : a_nxt + T::A_BYTES;
-      asm volatile("" : "+s"(ca.kt), "+s"(ca.soff), "+s"(a_cur), "+s"(a_nxt));
+      asm volatile("" : "+s"(ca.soff), "+s"(a_cur), "+s"(a_nxt));
     }
   };
   auto w_turn = [&]() __attribute__((always_inline)) {
-    if (cw.kt == ragged) w_pv = offset(params_again()->ldw, true);
-    if (cw.kt == nk) {
-      cw.kt = 0;
+    if (cw.soff == ragged) w_pv = offset(params_again()->ldw, true);
+    if (cw.soff == last + BK) {
       cw.soff = 0;
       ++cw.ord;
       w_tile();
-      if (ragged >= 0) w_pv = offset(params_again()->ldw, ragged == 0);
+      if (ragged == last) w_pv = offset(params_again()->ldw, nk == 1);
     }
-    asm volatile("" : "+s"(w_rs), "+s"(s_base), "+s"(s_bytes), "+s"(cw.soff), "+s"(cw.step), "+s"(cw.kt), "+s"(cw.ord), "+s"(dma_base), "+s"(dma_sc));
+    asm volatile("" : "+s"(w_rs), "+s"(s_base), "+s"(s_bytes), "+s"(cw.soff), "+s"(cw.step), "+s"(cw.ord), "+s"(dma_base), "+s"(dma_sc));
   };
   auto a_turn = [&]() __attribute__((always_inline)) {
-    if (ca.kt == ragged) a_pv = offset(params_again()->lda, true);
-    if (ca.kt == nk) {
-      ca.kt = 0;
+    if (ca.soff == ragged) a_pv = offset(params_again()->lda, true);
+    if (ca.soff == last + BK) {
       ca.soff = 0;
       ++ca.ord;
       a_tile();
-      if (ragged >= 0) a_pv = offset(params_again()->lda, ragged == 0);
+      if (ragged == last) a_pv = offset(params_again()->lda, nk == 1);
     }
-    asm volatile("" : "+s"(a_rs), "+s"(ca.soff), "+s"(ca.step), "+s"(ca.kt), "+s"(ca.ord), "+s"(a_cur), "+s"(a_nxt));
+    asm volatile("" : "+s"(a_rs), "+s"(ca.soff), "+s"(ca.step), "+s"(ca.ord), "+s"(a_cur), "+s"(a_nxt));
   };
 
   // ---- fragments: register set P (0 | 1) = NT W fragments, then MT A fragments, of 8 accumulator registers each ----
@@ -616,7 +613,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   auto step = [&](auto Pc) __attribute__((always_inline)) {
     if (kt == 0) block(Pc, IntC<1>{}, relaxed);
     else block(Pc, IntC<0>{}, false);
-    if (max(cw.kt, ca.kt) >= nk - 1) {
+    if (max(cw.soff, ca.soff) >= last) {
       w_turn();
       a_turn();
     }
