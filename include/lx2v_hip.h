@@ -436,7 +436,8 @@ int lx2v_quant_fp8_block128_f32(const float* w, int64_t ldw, uint8_t* out, int64
 
 /* ---- C[m, n] = epilogue(sum_b sa[m, b] sw[n / 128, b] (A8[m, b] . W8[n, b]) + bias[n]), bf16 out ----
  * b runs over the ceil(K / 128) blocks of K; sa[m, b] = a_scale[b * ld_a_scale + m], sw[i, b] = w_scale[i * ld_w_scale + b].
- * fp32 accumulation; epilogues as lx2v_gemm_bf16, with one rounding at the end (resid may alias C).
+ * sa * sw is formed first and has to be finite in fp32; fp32 accumulation; epilogues as lx2v_gemm_bf16, with one rounding at
+ * the end (resid may alias C).
  * K % 16 == 0, N % 8 == 0, e4m3 row strides % 16, all row strides of the matrices below 2^22 elements, any M >= 0.
  * A product of few output tiles is split along K: fp32 sums of each range in `workspace`
  * (lx2v_gemm_fp8_block128_workspace_bytes; 0: not split), joined in a fixed order by a second launch, so results repeat
