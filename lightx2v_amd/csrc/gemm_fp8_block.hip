@@ -17,6 +17,7 @@
 // weight rows straight into fragment registers, the waves split K.  Rows past M / N and columns past K arrive as zeros (range check of
 // the buffer descriptors).
 #include <algorithm>
+#include <atomic>
 
 #include "common.h"
 
@@ -734,14 +735,13 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void gemm_fp8_block_skinny_kerne
 }
 
 int device_cus() {
-  static int cus_cached[64];
-  int dev = 0, cus = 256;
-  if (hipGetDevice(&dev) == hipSuccess && dev >= 0 && dev < 64) {
-    if (cus_cached[dev] == 0) {
-      int v = 0;
-      cus_cached[dev] = (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && v > 0) ? v : 256;
-    }
-    cus = cus_cached[dev];
+  static std::atomic<int> cached[64];  // (calls from several threads at once may all ask: they store the same number)
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  int cus = cached[dev].load(std::memory_order_relaxed);
+  if (cus == 0) {
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) cus = 256;
+    cached[dev].store(cus, std::memory_order_relaxed);
   }
   return cus;
 }

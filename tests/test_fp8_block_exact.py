@@ -1,6 +1,8 @@
 """Block-scaled e4m3 Linear on operands whose sums are exact (oracle/fp8_block_ref.py: whole_operands): a correct product equals the 64-bit
 one rounded to bf16 bit for bit, and one lost column of K or one sum held in too few bits does not.  That these operands show such
 mistakes is checked on the CPU, with the mistakes made in the oracle."""
+import concurrent.futures
+
 import pytest
 import torch
 
@@ -119,3 +121,25 @@ def test_largest_row_strides(cuda, M, N, K):
         assert torch.equal(hip.gemm_fp8_block(*args, out=out, workspace=ws), v.to(torch.bfloat16))
         hip.gemm_fp8_block(*args, epilogue=hip.EPI_RESIDUAL, resid=resid, out=out, workspace=ws)
         assert torch.equal(out, (v + 3).to(torch.bfloat16))
+
+
+@pytest.mark.gpu
+def test_products_from_several_threads_at_once(cuda):
+    """Calls of different shapes from eight threads, each on its own stream: plan, workspace and error text are each call's own."""
+    shapes = [(13, 264, 1040), (40, 520, 4112), (300, 520, 2064), (900, 1288, 96)] * 2
+    sets = [_whole(*s, seed=i, device=cuda) for i, s in enumerate(shapes)]
+    want = [(a @ w.t().contiguous()).to(torch.bfloat16) for _, a, w in sets]
+    torch.cuda.synchronize()
+
+    def work(i):
+        q, same = sets[i][0], True
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(25):
+                same &= torch.equal(hip.gemm_fp8_block(*q), want[i])
+                with pytest.raises(hip.Lx2vError, match=f"K={16 * i + 8} "):   # refused: the text is this thread's own
+                    k = 16 * i + 8
+                    hip.gemm_fp8_block(*R.whole_operands(4, 8, k, 0, cuda))
+        return same
+
+    with concurrent.futures.ThreadPoolExecutor(8) as pool:
+        assert all(pool.map(work, range(8)))
